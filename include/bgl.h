@@ -64,6 +64,7 @@ enum {
     BGL_OP_COPY_LHS = 5, BGL_OP_COPY_RHS = 6
 };
 enum { BGL_RED_SUM = 0, BGL_RED_MAX = 1, BGL_RED_MIN = 2, BGL_RED_MEAN = 3 };
+enum { BGL_SCORE_SOFTMAX = 0, BGL_SCORE_SIGMOID = 1 };
 /* gspmm flags */
 enum {
     BGL_ZERO_INF = 1,  /* replace +-inf results with 0 (the max/min post-pass of
@@ -240,10 +241,84 @@ int bgl_gather_mm(const void *a, const void *b, const int64_t *idx_b, void *out,
                   int64_t d1, int64_t r, int64_t d2, int dtype, void *workspace,
                   size_t workspace_bytes, void *stream);
 
+/* Gradients of bgl_segment_mm (no counterpart in the reference, which has no
+ * backward pass): da[i] = grad[i] @ b[r]^T for the rows i of segment r, zero
+ * for rows past sum(seglen); db[r] = a[rows of r]^T @ grad[rows of r], zero
+ * for a segment without rows.  grad is (n, d2), a and da (n, d1), b and db
+ * (r, d1, d2), seglen a DEVICE int64 array of r entries, clamped as
+ * bgl_segment_mm clamps it.  da or db may be NULL: it is then not computed. */
+size_t bgl_segment_mm_backward_workspace_size(int64_t n, int64_t d1, int64_t r, int64_t d2,
+                                              int dtype);
+int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, const int64_t *seglen,
+                            int64_t n, int64_t d1, int64_t r, int64_t d2, void *da, void *db,
+                            int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Device-side status of the tensor-core grouped GEMM: 0, or the code of the
  * first bounded wait that expired (1-4) since the last call; synchronises
  * the device and clears the word. */
 int bgl_tc_error(void);
+
+/* ----------------------------------------- mixture-of-experts layer */
+/* Operators around the grouped products of a mixture-of-experts layer (no
+ * counterpart in the reference).
+ *
+ * Layer norm over the last axis of x (rows, d):
+ *   y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias
+ * weight and bias (d values) may be NULL, as may the outputs mean and rstd
+ * (rows values each).  wdtype is dtype, or BGL_F32 for bf16 rows; mean and rstd
+ * are float32, float64 for BGL_F64.  The backward call takes the mean and rstd
+ * of the forward one; dx, dweight, dbias may be NULL (not computed), dweight and
+ * dbias have wdtype.  The sums over rows have a fixed order. */
+int bgl_layer_norm(const void *x, const void *weight, const void *bias, int64_t rows, int64_t d,
+                   double eps, void *y, void *mean, void *rstd, int dtype, int wdtype,
+                   void *stream);
+size_t bgl_layer_norm_backward_workspace_size(int64_t rows, int64_t d, int dtype);
+int bgl_layer_norm_backward(const void *grad, const void *x, const void *mean, const void *rstd,
+                            const void *weight, int64_t rows, int64_t d, void *dx, void *dweight,
+                            void *dbias, int dtype, int wdtype, void *workspace,
+                            size_t workspace_bytes, void *stream);
+/* Routing: of logits (tokens, experts; BGL_F32 or BGL_BF16) the k best experts
+ * of each token, best first, ties to the lower expert.
+ *   s = softmax(logits) or sigmoid(logits),  c = s + bias (bias NULL: c = s)
+ * c only selects.  With num_groups > 1 the experts form that many equal runs; a
+ * group scores the sum of its group_top (1 or 2) best c, and only the
+ * topk_groups best groups are kept.  weights = scale * s of the chosen, first
+ * divided by their sum if renormalize is set.  Without a bias and without sums
+ * of c the order is the logits' own.  A logit of -inf (or c of -inf) masks its
+ * expert; a token with fewer than k experts left gets index -1 and weight 0 in
+ * the remaining places.  NaN ranks first, and makes the weights that depend on
+ * it NaN.  Limits: 1,024 experts, k <= 32, 32 groups.
+ * The backward call gives dlogits (logits' dtype) of the weights at the given
+ * indices; an index outside [0, experts) has no gradient. */
+int bgl_route_topk(const void *logits, const float *bias, int64_t tokens, int64_t experts,
+                   int64_t k, int score, int64_t num_groups, int64_t topk_groups, int group_top,
+                   int renormalize, double scale, float *weights, int64_t *indices, int dtype,
+                   void *stream);
+int bgl_route_topk_backward(const float *grad, const void *logits, const int64_t *indices,
+                            int64_t tokens, int64_t experts, int64_t k, int score, int renormalize,
+                            double scale, void *dlogits, int dtype, void *stream);
+/* The rows of (token, choice) pairs sorted by expert, equal ones in order:
+ * counts[e] = pairs of expert e, positions[i] = the row of pair i.  A pair whose
+ * index is outside [0, experts) goes to no expert: its row comes behind all
+ * others and is stored as ~row.  At most 8,191 experts, items < 2^31. */
+size_t bgl_expert_plan_workspace_size(int64_t items, int64_t experts);
+int bgl_expert_plan(const int64_t *indices, int64_t items, int64_t experts, int64_t *counts,
+                    int32_t *positions, void *workspace, size_t workspace_bytes, void *stream);
+/* With positions (tokens, k) of a plan, p = positions[t, j]:
+ *   dispatch:  rows[p] = x[t]           (zeros at ~p of a pair without expert)
+ *   combine:   y[t] = sum_j weights[t, j] * rows[p]   (weights NULL: 1)
+ *   backward:  drows[p] = weights[t, j] * grad[t],  dweights[t, j] = <grad[t], rows[p]>
+ * Pairs without expert add nothing, their drows are zeros and their dweights 0.
+ * weights and dweights are float32, float64 for BGL_F64; drows and dweights may
+ * be NULL.  The gradient of dispatch is combine without weights.  Positions that
+ * no plan gives (outside the rows) are skipped. */
+int bgl_dispatch_rows(const void *x, const int32_t *positions, int64_t tokens, int64_t k,
+                      int64_t d, void *rows, int dtype, void *stream);
+int bgl_combine_rows(const void *rows, const int32_t *positions, const void *weights,
+                     int64_t tokens, int64_t k, int64_t d, void *y, int dtype, void *stream);
+int bgl_combine_rows_backward(const void *grad, const void *rows, const int32_t *positions,
+                              const void *weights, int64_t tokens, int64_t k, int64_t d,
+                              void *drows, void *dweights, int dtype, void *stream);
 
 /* ------------------------------------------------ multi-GPU halo buffers */
 /* Device buffers shared between the processes of one node (one process per

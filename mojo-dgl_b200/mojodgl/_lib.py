@@ -28,6 +28,7 @@ TARGETS = {"u": SRC_CODE, "v": DST_CODE, "e": EDGE_CODE}
 
 # include/bgl.h
 BGL_F32, BGL_F64, BGL_BF16 = 0, 1, 2
+SCORES = {"softmax": 0, "sigmoid": 1}
 BGL_ZERO_INF = 1
 BGL_ACCUMULATE = 2
 
@@ -67,7 +68,23 @@ SIGNATURES = {
     "bgl_segment_mm": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _P, _SZ, _P], _INT),
     "bgl_gather_mm_workspace_size": ([_I64, _I64, _I64, _I64, _INT], _SZ),
     "bgl_gather_mm": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _P, _SZ, _P], _INT),
+    "bgl_segment_mm_backward_workspace_size": ([_I64, _I64, _I64, _I64, _INT], _SZ),
+    "bgl_segment_mm_backward": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _SZ, _P],
+                                _INT),
     "bgl_tc_error": ([], _INT),
+    "bgl_layer_norm": ([_P, _P, _P, _I64, _I64, ctypes.c_double, _P, _P, _P, _INT, _INT, _P], _INT),
+    "bgl_layer_norm_backward_workspace_size": ([_I64, _I64, _INT], _SZ),
+    "bgl_layer_norm_backward": ([_P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _INT, _INT, _P, _SZ,
+                                 _P], _INT),
+    "bgl_route_topk": ([_P, _P, _I64, _I64, _I64, _INT, _I64, _I64, _INT, _INT, ctypes.c_double,
+                        _P, _P, _INT, _P], _INT),
+    "bgl_route_topk_backward": ([_P, _P, _P, _I64, _I64, _I64, _INT, _INT, ctypes.c_double, _P,
+                                 _INT, _P], _INT),
+    "bgl_expert_plan_workspace_size": ([_I64, _I64], _SZ),
+    "bgl_expert_plan": ([_P, _I64, _I64, _P, _P, _P, _SZ, _P], _INT),
+    "bgl_dispatch_rows": ([_P, _P, _I64, _I64, _I64, _P, _INT, _P], _INT),
+    "bgl_combine_rows": ([_P, _P, _P, _I64, _I64, _I64, _P, _INT, _P], _INT),
+    "bgl_combine_rows_backward": ([_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _INT, _P], _INT),
     "bgl_cumsum_workspace_size": ([_I64], _SZ),
     "bgl_cumsum_i64": ([_P, _P, _I64, _P, _SZ, _P], _INT),
     "bgl_clamp_i64": ([_P, _P, _I64, _I64, _I64, _P], _INT),

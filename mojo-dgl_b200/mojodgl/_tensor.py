@@ -136,6 +136,37 @@ def to_dev(a, dtype: torch.dtype = None) -> torch.Tensor:
     return t.to(dev)
 
 
+def array(a):
+    """The operand with a shape and an element type: lists become numpy arrays."""
+    return a if a is None or is_torch(a) else np.asanyarray(a)
+
+
+def is_bf16(a) -> bool:
+    return is_torch(a) and a.dtype == torch.bfloat16
+
+
+def is_f32(a) -> bool:
+    return a.dtype == (torch.float32 if is_torch(a) else np.float32)
+
+
+def float_type(*xs):
+    """bfloat16 if every operand is a bfloat16 tensor, else ``common_float`` of
+    the operands under the ``feature`` rules."""
+    if all(is_bf16(x) for x in xs):
+        return torch.bfloat16
+    return common_float(*(feature(x) for x in xs))
+
+
+def on(dev: torch.device, a, dtype: torch.dtype):
+    """``to_dev`` for an operand that may be absent (None), with what is already
+    there as asked returned as it is."""
+    if a is None:
+        return None
+    if is_torch(a) and a.dtype == dtype and a.device == dev and a.is_contiguous():
+        return a
+    return to_dev(a, dtype)
+
+
 def result(t: torch.Tensor, kind: int):
     """Hand a device result back in the caller's kind."""
     if kind == TORCH_CUDA:

@@ -1,0 +1,116 @@
+"""Layer norm over the last axis, forward and backward.
+
+The reference has no dense layers; a graph transformer or mixture-of-experts
+block runs its norm next to this package's grouped products, on the same
+arrays.  bfloat16 tensors stay bfloat16 (statistics and sums in float32);
+weight and bias may then be float32 or bfloat16.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _tensor as T
+from .._lib import check, lib
+from ..base import DGLError
+
+__all__ = ["layer_norm", "layer_norm_backward"]
+
+
+def _types(x, *params):
+    """Element types of the rows and of the parameters."""
+    present = [p for p in params if p is not None]
+    if T.is_bf16(x) and all(T.is_bf16(p) or T.is_f32(p) for p in present):
+        narrow = present and all(T.is_bf16(p) for p in present)
+        return torch.bfloat16, torch.bfloat16 if narrow else torch.float32
+    dtype = T.common_float(*(T.feature(v) for v in (x, *present)))
+    return dtype, dtype
+
+
+def _stat_type(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _check_rows(x, *params):
+    shape = T.shape_of(x)
+    if not shape or shape[-1] < 1:
+        raise DGLError("layer norm needs a last axis of at least one value, got shape {}".format(shape))
+    for name, p in params:
+        if p is not None and T.shape_of(p) != (shape[-1],):
+            raise DGLError("{} must have shape ({},), got {}".format(name, shape[-1], T.shape_of(p)))
+    d = int(shape[-1])
+    rows = 1
+    for s in shape[:-1]:
+        rows *= int(s)
+    return shape, rows, d
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
+    r"""``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis.
+
+    ``x`` is (..., D); ``weight`` and ``bias`` are (D,), a bias only together
+    with a weight.  Returns an array shaped like ``x``; with ``return_stats``
+    also the mean and 1 / sqrt(var + eps) of every row, which
+    :func:`layer_norm_backward` takes.
+    """
+    if bias is not None and weight is None:
+        raise DGLError("layer_norm takes a bias only together with a weight")
+    if not eps >= 0:
+        raise DGLError("eps must not be negative, got {}".format(eps))
+    kind = T.kind_of(x, weight, bias)
+    x, weight, bias = T.array(x), T.array(weight), T.array(bias)
+    shape, rows, d = _check_rows(x, ("weight", weight), ("bias", bias))
+    dtype, wdtype = _types(x, weight, bias)
+    dev = T.device()
+    xt, wt, bt = T.on(dev, x, dtype), T.on(dev, weight, wdtype), T.on(dev, bias, wdtype)
+    y = torch.empty(shape, dtype=dtype, device=dev)
+    mean = rstd = None
+    if return_stats:
+        mean = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
+        rstd = torch.empty_like(mean)
+    check(lib().bgl_layer_norm(T.ptr(xt), T.ptr(wt), T.ptr(bt), rows, d, float(eps), T.ptr(y),
+                               T.ptr(mean), T.ptr(rstd), T.code_of(dtype), T.code_of(wdtype),
+                               T.stream()), "layer_norm")
+    if not return_stats:
+        return T.result(y, kind)
+    return T.result(y, kind), T.result(mean, kind), T.result(rstd, kind)
+
+
+def layer_norm_backward(grad, x, mean, rstd, weight=None):
+    r"""Gradients of :func:`layer_norm` with respect to x, weight and bias.
+
+    ``grad`` is shaped like ``x``; ``mean`` and ``rstd`` are the forward
+    call's.  Returns ``(dx, dweight, dbias)``, the last two None without a
+    weight.  The sums over rows have a fixed order: the same inputs give the
+    same bits.
+    """
+    kind = T.kind_of(grad, x, mean, rstd, weight)
+    grad, x, mean, rstd, weight = (T.array(v) for v in (grad, x, mean, rstd, weight))
+    shape, rows, d = _check_rows(x, ("weight", weight))
+    if T.shape_of(grad) != shape:
+        raise DGLError("grad must have the shape of x, {}, got {}".format(shape, T.shape_of(grad)))
+    for name, s in (("mean", mean), ("rstd", rstd)):
+        if T.shape_of(s) != shape[:-1]:
+            raise DGLError("{} must have shape {}, got {}".format(name, shape[:-1], T.shape_of(s)))
+    if T.is_bf16(x) and T.is_bf16(grad):
+        dtype, wdtype = _types(x, weight)
+    else:
+        dtype = wdtype = T.common_float(*(T.feature(v) for v in (x, grad, weight) if v is not None))
+    dev = T.device()
+    gt, xt = T.on(dev, grad, dtype), T.on(dev, x, dtype)
+    mt, rt = T.on(dev, mean, _stat_type(dtype)), T.on(dev, rstd, _stat_type(dtype))
+    wt = T.on(dev, weight, wdtype)
+    dx = torch.empty(shape, dtype=dtype, device=dev)
+    dw = db = ws = None
+    nbytes = 0
+    if weight is not None:
+        dw, db = torch.empty((2, d), dtype=wdtype, device=dev).unbind(0)
+        nbytes = lib().bgl_layer_norm_backward_workspace_size(rows, d, T.code_of(dtype))
+        ws = T.workspace(nbytes)
+    check(lib().bgl_layer_norm_backward(T.ptr(gt), T.ptr(xt), T.ptr(mt), T.ptr(rt), T.ptr(wt), rows,
+                                        d, T.ptr(dx), T.ptr(dw), T.ptr(db), T.code_of(dtype),
+                                        T.code_of(wdtype), T.ptr(ws), nbytes, T.stream()),
+          "layer_norm_backward")
+    if weight is None:
+        return T.result(dx, kind), None, None
+    return T.result(dx, kind), T.result(dw, kind), T.result(db, kind)

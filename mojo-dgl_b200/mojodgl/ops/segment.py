@@ -18,7 +18,7 @@ from .._lib import BGL_ZERO_INF, OP_COPY_RHS, REDUCERS, check, lib
 from ..base import DGLError
 from .sddmm import flat_feature, out_shape
 
-__all__ = ["segment_reduce", "segment_softmax", "segment_mm"]
+__all__ = ["segment_reduce", "segment_softmax", "segment_mm", "segment_mm_backward"]
 
 
 def _offsets(seglen):
@@ -144,3 +144,45 @@ def segment_mm(a, b, seglen_a):
                                   T.ptr(ws), nbytes, T.stream())
         check(rc, "segment_mm")
     return T.result(out, kind)
+
+
+def segment_mm_backward(grad, a, b, seglen_a, need_a=True, need_b=True):
+    r"""Gradients of :func:`segment_mm` with respect to ``a`` and ``b``.
+
+    ``grad`` is (N, D2), the other arguments are the forward call's.  Returns
+    ``(da, db)``: ``da[i] = grad[i] @ b[r].T`` for the rows i of segment r (rows
+    past ``sum(seglen_a)`` are zero) and ``db[r] = a[rows of r].T @ grad[rows of
+    r]``; the one that is not needed is None.  A ``seglen_a`` on the device is
+    not read back: negative lengths count as 0 there, and no segment runs past
+    N.  bfloat16 tensors run in BF16 with float32 sums, float32 and float64
+    exactly.
+    """
+    kind = T.kind_of(grad, a, b, seglen_a)
+    grad, a, b = T.array(grad), T.array(a), T.array(b)
+    if len(T.shape_of(a)) != 2 or len(T.shape_of(b)) != 3:
+        raise DGLError("segment_mm_backward wants a 2-D left operand and a 3-D right operand")
+    n, d1 = (int(v) for v in T.shape_of(a))
+    r, b_d1, d2 = (int(v) for v in T.shape_of(b))
+    if b_d1 != d1:
+        raise DGLError("inner dimensions do not match: {} vs {}".format(d1, b_d1))
+    if T.shape_of(grad) != (n, d2):
+        raise DGLError("grad must be ({}, {}), got shape {}".format(n, d2, T.shape_of(grad)))
+    dtype = T.float_type(grad, a, b)
+    seg = T.ids(seglen_a)
+    if T.shape_of(seg) != (r,):
+        raise DGLError("seglen_a must have one entry per b block: {} != {}".format(T.shape_of(seg), r))
+    if not (T.is_torch(seg) and seg.is_cuda) and r and (int(seg.min()) < 0 or int(seg.sum()) > n):
+        raise DGLError("segment lengths must be non-negative and sum to {}, got a minimum of "
+                       "{} and a sum of {}".format(n, int(seg.min()), int(seg.sum())))
+    dev = T.device()
+    gt, at, bt = T.on(dev, grad, dtype), T.on(dev, a, dtype), T.on(dev, b, dtype)
+    st = T.on(dev, seg, torch.int64)
+    da = torch.empty((n, d1), dtype=dtype, device=dev) if need_a else None
+    db = torch.empty((r, d1, d2), dtype=dtype, device=dev) if need_b else None
+    code = T.code_of(dtype)
+    nbytes = lib().bgl_segment_mm_backward_workspace_size(n, d1, r, d2, code)
+    ws = T.workspace(nbytes)
+    check(lib().bgl_segment_mm_backward(T.ptr(gt), T.ptr(at), T.ptr(bt), T.ptr(st), n, d1, r, d2,
+                                        T.ptr(da), T.ptr(db), code, T.ptr(ws), nbytes, T.stream()),
+          "segment_mm_backward")
+    return T.result(da, kind) if need_a else None, T.result(db, kind) if need_b else None
