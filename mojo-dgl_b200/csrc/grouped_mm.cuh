@@ -27,10 +27,38 @@ struct GmmLayout {
 GmmLayout gmm_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype,
                      bool gather);
 
-// tcgen05 path (grouped_mm_tc.cu).
+// tcgen05 path (grouped_mm_tc.cu).  With b == nullptr, l.tc_b already is the
+// K-major B: r blocks of d2 rows of d1 values.
 bool gmm_tensor_core_supported(int64_t d1, int64_t d2, int dtype);
 bool gmm_tensor_core_fits(int64_t n, int64_t r, int64_t d2);
 int gmm_tensor_core(const void *a, const void *b, void *out, const GmmLayout &l, int64_t n,
                     int64_t d1, int64_t r, int64_t d2, int dtype, cudaStream_t s);
+
+// Schedule of the gradients (grouped_mm_grad.cu writes it, one kernel, in the
+// caller's workspace).
+struct GradLayout {
+    int64_t *off;       // [r + 1] first row of each segment
+    int64_t *tile_off;  // [r + 1] first 128-row tile of each segment (da)
+    int64_t *unit_off;  // [r + 1] first unit of each segment (db)
+    int64_t *mode;      // [1] 1: db's units are split evenly over the CTAs
+    float *partial;     // db: partial tiles of split units
+    size_t bytes;
+};
+
+// tcgen05 path of db (grouped_mm_grad_tc.cu).  A unit is one 64-row slice of
+// one output tile's sum; a segment without rows has one unit a tile.
+struct GradTiles {
+    int64_t tiles_n;      // 256-column tiles of a segment's block
+    int64_t per_segment;  // 256 x 256 tiles of a segment's block
+    int ctas;
+};
+constexpr int kGradSlice = 64, kGradTile = 256;
+bool gmm_grad_tc_supported(const void *grad, const void *a, const void *db, int64_t n, int64_t d1,
+                           int64_t r, int64_t d2, int dtype);
+GradTiles gmm_grad_tiles(int64_t n, int64_t d1, int64_t r, int64_t d2);
+int gmm_grad_tensor_core(const void *grad, const void *a, void *db, const GradLayout &l,
+                         const GradTiles &t, int64_t n, int64_t d1, int64_t r, int64_t d2,
+                         cudaStream_t s);
+cudaError_t gmm_grad_tc_error(int *code);
 
 }  // namespace bgl

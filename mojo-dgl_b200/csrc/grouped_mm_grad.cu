@@ -4,6 +4,7 @@
 //   da[i] = dout[i] @ b[r(i)]^T        db[r] = a[rows of r]^T @ dout[rows of r]
 //
 // Rows past the last segment have da = 0; a segment without rows has db = 0.
+#include "grouped_mm.cuh"
 #include "rows.cuh"
 
 namespace bgl {
@@ -11,18 +12,96 @@ namespace {
 
 constexpr int kTile = 64, kDepth = 16;
 
-// First row of each segment, clamped as segment_mm's own schedule clamps:
-// negative lengths count as 0 and no segment runs past n.
-__global__ void k_segment_offsets(const int64_t *__restrict__ seglen, int64_t r, int64_t n,
-                                  int64_t *__restrict__ off) {
-    if (blockIdx.x != 0 || threadIdx.x != 0) return;
-    int64_t row = 0;
-    off[0] = 0;
-    for (int64_t i = 0; i < r; ++i) {
-        int64_t len = seglen[i] < 0 ? 0 : seglen[i];
-        row += len < n - row ? len : n - row;
-        off[i + 1] = row;
+// Sum over the block's earlier threads (exclusive), and over all of them.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warps, int64_t &total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockDim.x >> 5;
+    int64_t sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
     }
+    if (lane == 31) warps[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+        int64_t w = lane < n ? warps[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += up;
+        }
+        warps[lane] = w;
+    }
+    __syncthreads();
+    total = warps[n - 1];
+    const int64_t before = (warp ? warps[warp - 1] : 0) + sum - v;
+    __syncthreads();
+    return before;
+}
+
+// First row, first 128-row tile and first unit of each segment, one block.
+// The rows are clamped as segment_mm's own schedule clamps them: negative
+// lengths count as 0 and no segment runs past n.
+//
+// mode: db's tiles go round robin to the CTAs where that is even enough, else
+// all units are split evenly (a tile cut between CTAs is then joined from
+// partial tiles).  Both makespans are counted in units of one 64-row slice.
+__global__ void __launch_bounds__(1024)
+    k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, int64_t per_segment,
+                    int ctas, GradLayout l) {
+    __shared__ int64_t warps[32];
+    int64_t rows = 0, tiles = 0, units = 0;
+    for (int64_t i0 = 0; i0 < r; i0 += blockDim.x) {
+        const int64_t i = i0 + threadIdx.x;
+        int64_t len = i < r ? seglen[i] : 0, total;
+        len = len < 0 ? 0 : len < n ? len : n;
+        const int64_t row = rows + block_scan(len, warps, total);
+        const int64_t first = row < n ? row : n, end = row + len < n ? row + len : n;
+        rows += total;
+        const int64_t slices = (end - first + kGradSlice - 1) / kGradSlice;
+        const int64_t row_tiles = (end - first + 127) / 128;
+        const int64_t tile = tiles + block_scan(row_tiles, warps, total);
+        tiles += total;
+        const int64_t mine = i < r ? (slices ? slices : 1) * per_segment : 0;
+        const int64_t unit = units + block_scan(mine, warps, total);
+        units += total;
+        if (i < r) {
+            l.off[i] = first;
+            l.tile_off[i] = tile;
+            l.unit_off[i] = unit;
+        }
+    }
+    if (threadIdx.x == 0) {
+        l.off[r] = rows < n ? rows : n;
+        l.tile_off[r] = tiles;
+        l.unit_off[r] = units;
+        *l.mode = 0;
+    }
+    __syncthreads();
+    if (ctas < 1) return;
+    // CTA c's units when it takes the tiles c, c + ctas, ...; writing out a
+    // tile costs about as much as kTileCost units, joining one more
+    constexpr int64_t kTileCost = 6, kJoinCost = 20;
+    const int64_t all = r * per_segment;
+    int64_t most = 0;
+    if (threadIdx.x < ctas && all <= 64 * (int64_t)ctas) {
+        for (int64_t w = threadIdx.x; w < all; w += ctas) {
+            const int64_t seg = w / per_segment;
+            most += (l.unit_off[seg + 1] - l.unit_off[seg]) / per_segment + kTileCost;
+        }
+    }
+    const int64_t even = units / ctas + (all / ctas + 2) * kTileCost + kJoinCost;
+    if (most > even) *l.mode = 1;
+}
+
+// Rows past the last segment: da = 0.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_zero_rows(T *__restrict__ da, const int64_t *__restrict__ off, int64_t r, int64_t n,
+                int64_t d1) {
+    for (int64_t i = off[r] * d1 + blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n * d1;
+         i += (int64_t)gridDim.x * blockDim.x)
+        da[i] = from_acc<T>(0);
 }
 
 // 64 x 64 outputs a block of 256 threads, 4 x 4 a thread, over a shared strip
@@ -158,6 +237,21 @@ int simt(const void *g, const void *a, const void *b, const int64_t *off, int64_
     return BGL_OK;
 }
 
+GradLayout grad_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype) {
+    Carver c(ws);
+    GradLayout l;
+    l.off = c.take<int64_t>((size_t)r + 1);
+    l.tile_off = c.take<int64_t>((size_t)r + 1);
+    l.unit_off = c.take<int64_t>((size_t)r + 1);
+    l.mode = c.take<int64_t>(1);
+    // two partial tiles a CTA: the one it begins with and the one it ends with
+    l.partial = dtype == BGL_BF16
+                    ? c.take<float>((size_t)gmm_grad_tiles(n, d1, r, d2).ctas * 2 * kGradTile * kGradTile)
+                    : nullptr;
+    l.bytes = c.used + 256;
+    return l;
+}
+
 }  // namespace
 }  // namespace bgl
 
@@ -168,7 +262,7 @@ extern "C" {
 size_t bgl_segment_mm_backward_workspace_size(int64_t n, int64_t d1, int64_t r, int64_t d2,
                                               int dtype) {
     if (n < 0 || r < 0 || d1 < 0 || d2 < 0) return 0;
-    return (size_t)(r + 1) * sizeof(int64_t) + 256;
+    return grad_layout(nullptr, n, d1, r, d2, dtype).bytes;
 }
 
 int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, const int64_t *seglen,
@@ -177,22 +271,47 @@ int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, cons
     const char *who = "bgl_segment_mm_backward";
     if (!row_dtype(dtype)) return fail(BGL_E_UNSUPPORTED, "%s: dtype %d", who, dtype);
     if (n < 0 || d1 < 0 || r < 0 || d2 < 0) return fail(BGL_E_INVALID, "%s: negative size", who);
-    if (n >= (int64_t(1) << 31) || d1 >= (1 << 22) || d2 >= (1 << 22))
-        return fail(BGL_E_UNSUPPORTED, "%s: n >= 2^31 or a width >= 2^22", who);
+    if (n >= (int64_t(1) << 31) || r >= (int64_t(1) << 31) || d1 >= (1 << 22) || d2 >= (1 << 22))
+        return fail(BGL_E_UNSUPPORTED, "%s: n or r >= 2^31 or a width >= 2^22", who);
     if (!da && !db) return BGL_OK;
     if (r && !seglen) return fail(BGL_E_INVALID, "%s: null seglen", who);
     if (da && n && d1 && d2 && (!grad || (r && !b))) return fail(BGL_E_INVALID, "%s: null buffer", who);
     if (db && n && r && d1 && d2 && (!grad || !a)) return fail(BGL_E_INVALID, "%s: null buffer", who);
-    if (!workspace || workspace_bytes < bgl_segment_mm_backward_workspace_size(n, d1, r, d2, dtype))
+    GradLayout l = grad_layout(workspace, n, d1, r, d2, dtype);
+    if (!workspace || workspace_bytes < l.bytes)
         return fail(BGL_E_WORKSPACE, "%s: workspace too small", who);
     cudaStream_t s = as_stream(stream);
-    Carver c(workspace);
-    int64_t *off = c.take<int64_t>((size_t)r + 1);
-    k_segment_offsets<<<1, 32, 0, s>>>(seglen, r, n, off);
+    const bool want_da = da && n && d1, want_db = db && r && d1 && d2;
+    const bool da_tc = want_da && dtype == BGL_BF16 && r && d2 &&
+                       gmm_tensor_core_supported(d2, d1, dtype) && gmm_tensor_core_fits(n, r, d1) &&
+                       aligned(grad, 16) && aligned(b, 16) && aligned(da, 16);
+    const bool db_tc = want_db && gmm_grad_tc_supported(grad, a, db, n, d1, r, d2, dtype);
+    const GradTiles t = gmm_grad_tiles(n, d1, r, d2);
+    k_grad_schedule<<<1, 1024, 0, s>>>(seglen, r, n, t.per_segment, db_tc ? t.ctas : 0, l);
     BGL_LAUNCH_CHECK();
-    if (dtype == BGL_F64) return simt<double>(grad, a, b, off, n, d1, r, d2, da, db, s);
-    if (dtype == BGL_F32) return simt<float>(grad, a, b, off, n, d1, r, d2, da, db, s);
-    return simt<__nv_bfloat16>(grad, a, b, off, n, d1, r, d2, da, db, s);
+    if (da_tc) {
+        const int64_t blocks = (n * d1 + 255) / 256, cap = (int64_t)num_sms() * 8;
+        k_zero_rows<__nv_bfloat16><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, s>>>(
+            (__nv_bfloat16 *)da, l.off, r, n, d1);
+        BGL_LAUNCH_CHECK();
+        // b[r] is (d1, d2): rows of the product's columns, already K-major
+        GmmLayout g = {};
+        g.seg_off = l.off;
+        g.tile_off = l.tile_off;
+        g.tc_b = const_cast<void *>(b);
+        const int rc = gmm_tensor_core(grad, nullptr, da, g, n, d2, r, d1, dtype, s);
+        if (rc) return rc;
+    }
+    if (db_tc) {
+        const int rc = gmm_grad_tensor_core(grad, a, db, l, t, n, d1, r, d2, s);
+        if (rc) return rc;
+    }
+    if (da_tc || !want_da) da = nullptr;
+    if (db_tc || !want_db) db = nullptr;
+    if (!da && !db) return BGL_OK;
+    if (dtype == BGL_F64) return simt<double>(grad, a, b, l.off, n, d1, r, d2, da, db, s);
+    if (dtype == BGL_F32) return simt<float>(grad, a, b, l.off, n, d1, r, d2, da, db, s);
+    return simt<__nv_bfloat16>(grad, a, b, l.off, n, d1, r, d2, da, db, s);
 }
 
 }  // extern "C"
