@@ -27,38 +27,57 @@ struct GmmLayout {
 GmmLayout gmm_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype,
                      bool gather);
 
-// tcgen05 path (grouped_mm_tc.cu).  With b == nullptr, l.tc_b already is the
-// K-major B: r blocks of d2 rows of d1 values.
+// tcgen05 path (grouped_mm_tc.cu).
 bool gmm_tensor_core_supported(int64_t d1, int64_t d2, int dtype);
 bool gmm_tensor_core_fits(int64_t n, int64_t r, int64_t d2);
 int gmm_tensor_core(const void *a, const void *b, void *out, const GmmLayout &l, int64_t n,
                     int64_t d1, int64_t r, int64_t d2, int dtype, cudaStream_t s);
 
-// Schedule of the gradients (grouped_mm_grad.cu writes it, one kernel, in the
-// caller's workspace).
+// Gradients of the grouped product on the tensor cores (grouped_mm_grad_tc.cu).
+// Work comes in items: 256 x 256 tiles of da, and pieces of db's 256 x 256
+// tiles (a range of the segment's 64-row slices).
+constexpr int kGradSlice = 64, kGradTile = 256;
+
+// The schedule, written by one kernel into the caller's workspace.  Segments
+// are in the order of `order` in the arrays of db.
 struct GradLayout {
     int64_t *off;       // [r + 1] first row of each segment
-    int64_t *tile_off;  // [r + 1] first 128-row tile of each segment (da)
-    int64_t *unit_off;  // [r + 1] first unit of each segment (db)
-    int64_t *mode;      // [1] 1: db's units are split evenly over the CTAs
-    float *partial;     // db: partial tiles of split units
+    int64_t *row_off;   // [r + 1] first 256-row tile of each segment (da)
+    int32_t *order;     // [r] db's segments, long ones first
+    int64_t *item_off;  // [r + 1] db's items before those of order[i]
+    int64_t *cut_off;   // [r + 1] db's tiles of several pieces before those of order[i]
+    int64_t *slot_off;  // [r + 1] their partial tiles
+    int64_t *head;      // [kHead] see k_grad_schedule
+    float *partial;     // partial tiles
     size_t bytes;
 };
+enum { kHeadItems = 0, kHeadDbItems = 1, kHeadPiece = 2, kHeadCut = 3, kHeadNext = 4, kHead = 5 };
 
-// tcgen05 path of db (grouped_mm_grad_tc.cu).  A unit is one 64-row slice of
-// one output tile's sum; a segment without rows has one unit a tile.
+// How a db tile's slices are cut: `count` pieces of `slices` each, the last
+// one maybe shorter.
+struct GradPieces {
+    int64_t count, slices;
+};
+__host__ __device__ inline GradPieces grad_pieces(int64_t rows, int64_t most) {
+    const int64_t all = rows > 0 ? (rows + kGradSlice - 1) / kGradSlice : 1;
+    const int64_t count = (all + most - 1) / most, slices = (all + count - 1) / count;
+    return {(all + slices - 1) / slices, slices};
+}
+
 struct GradTiles {
-    int64_t tiles_n;      // 256-column tiles of a segment's block
-    int64_t per_segment;  // 256 x 256 tiles of a segment's block
+    int64_t tiles1, tiles2;  // 256-column tiles of d1 and d2
     int ctas;
 };
-constexpr int kGradSlice = 64, kGradTile = 256;
-bool gmm_grad_tc_supported(const void *grad, const void *a, const void *db, int64_t n, int64_t d1,
-                           int64_t r, int64_t d2, int dtype);
 GradTiles gmm_grad_tiles(int64_t n, int64_t d1, int64_t r, int64_t d2);
-int gmm_grad_tensor_core(const void *grad, const void *a, void *db, const GradLayout &l,
-                         const GradTiles &t, int64_t n, int64_t d1, int64_t r, int64_t d2,
-                         cudaStream_t s);
+// At most this many partial tiles a CTA (k_grad_schedule's rule keeps to it).
+constexpr int kGradSlots = 4;
+
+// da or db may be null (not wanted).
+bool gmm_grad_tc_supported(const void *grad, const void *a, const void *b, const void *da,
+                           const void *db, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype);
+int gmm_grad_tensor_core(const void *grad, const void *a, const void *b, void *da, void *db,
+                         const GradLayout &l, const GradTiles &t, int64_t n, int64_t d1, int64_t r,
+                         int64_t d2, cudaStream_t s);
 cudaError_t gmm_grad_tc_error(int *code);
 
 }  // namespace bgl

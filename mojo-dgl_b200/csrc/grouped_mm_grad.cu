@@ -39,18 +39,25 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warps, int64_t
     return before;
 }
 
-// First row, first 128-row tile and first unit of each segment, one block.
+// First row and first 256-row tile of each segment, and db's items; one block.
 // The rows are clamped as segment_mm's own schedule clamps them: negative
 // lengths count as 0 and no segment runs past n.
 //
-// mode: db's tiles go round robin to the CTAs where that is even enough, else
-// all units are split evenly (a tile cut between CTAs is then joined from
-// partial tiles).  Both makespans are counted in units of one 64-row slice.
+// Items are taken by whichever CTA is free, db's first and its long segments
+// first, da's small tiles last, so the CTAs end together.  A db tile is cut
+// into pieces only where its sum would outlast the rest: its pieces have at
+// most (da's work + half of db's) / CTAs slices, which also bounds the partial
+// tiles (a sum of L slices cut into pieces of P has ceil(L / P) < 2 L / P of
+// them where L > P, all sums together 2 * work / P <= 4 a CTA).  A tile's
+// read-out counts as kTileCost slices (2.4 us against 0.55 us a slice).
 __global__ void __launch_bounds__(1024)
-    k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, int64_t per_segment,
-                    int ctas, GradLayout l) {
+    k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, GradTiles t,
+                    int64_t slices2, bool want_da, bool want_db, GradLayout l) {
+    constexpr int64_t kTileCost = 4, kShortest = 8;
+    constexpr int kSorted = 256;  // more segments than this stay in order
     __shared__ int64_t warps[32];
-    int64_t rows = 0, tiles = 0, units = 0;
+    __shared__ int64_t lens[kSorted];
+    int64_t rows = 0, tiles = 0, slices = 0;
     for (int64_t i0 = 0; i0 < r; i0 += blockDim.x) {
         const int64_t i = i0 + threadIdx.x;
         int64_t len = i < r ? seglen[i] : 0, total;
@@ -58,50 +65,70 @@ __global__ void __launch_bounds__(1024)
         const int64_t row = rows + block_scan(len, warps, total);
         const int64_t first = row < n ? row : n, end = row + len < n ? row + len : n;
         rows += total;
-        const int64_t slices = (end - first + kGradSlice - 1) / kGradSlice;
-        const int64_t row_tiles = (end - first + 127) / 128;
-        const int64_t tile = tiles + block_scan(row_tiles, warps, total);
+        const int64_t tile = tiles + block_scan((end - first + kGradTile - 1) / kGradTile, warps, total);
         tiles += total;
-        const int64_t mine = i < r ? (slices ? slices : 1) * per_segment : 0;
-        const int64_t unit = units + block_scan(mine, warps, total);
-        units += total;
+        int64_t mine = (end - first + kGradSlice - 1) / kGradSlice;
+        if (i < r && mine == 0) mine = 1;  // a segment without rows: one piece a tile writes zeros
+        block_scan(mine, warps, total);
+        slices += total;
         if (i < r) {
             l.off[i] = first;
-            l.tile_off[i] = tile;
-            l.unit_off[i] = unit;
+            l.row_off[i] = tile;
+            if (r <= kSorted) lens[i] = mine;
         }
     }
     if (threadIdx.x == 0) {
         l.off[r] = rows < n ? rows : n;
-        l.tile_off[r] = tiles;
-        l.unit_off[r] = units;
-        *l.mode = 0;
+        l.row_off[r] = tiles;
     }
     __syncthreads();
-    if (ctas < 1) return;
-    // CTA c's units when it takes the tiles c, c + ctas, ...; writing out a
-    // tile costs about as much as kTileCost units, joining one more
-    constexpr int64_t kTileCost = 6, kJoinCost = 20;
-    const int64_t all = r * per_segment;
-    int64_t most = 0;
-    if (threadIdx.x < ctas && all <= 64 * (int64_t)ctas) {
-        for (int64_t w = threadIdx.x; w < all; w += ctas) {
-            const int64_t seg = w / per_segment;
-            most += (l.unit_off[seg + 1] - l.unit_off[seg]) / per_segment + kTileCost;
+    if (!want_da && !want_db) return;
+    for (int64_t i = threadIdx.x; i < r; i += blockDim.x) {
+        int64_t at = i;
+        if (r <= kSorted) {
+            at = 0;
+            for (int j = 0; j < (int)r; ++j) at += lens[j] > lens[i] || (lens[j] == lens[i] && j < i);
+        }
+        l.order[at] = (int32_t)i;
+    }
+    __syncthreads();
+    const int64_t per_segment = t.tiles1 * t.tiles2;
+    const int64_t da_items = want_da ? tiles * t.tiles1 : 0;
+    const int64_t da_work = da_items * (slices2 + kTileCost);
+    const int64_t db_work = slices * per_segment;
+    int64_t piece = (da_work + db_work / 2 + t.ctas - 1) / t.ctas;
+    if (piece < kShortest) piece = kShortest;
+    int64_t items = 0, cut = 0, slots = 0;
+    for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {
+        const int64_t k = k0 + threadIdx.x;
+        int64_t pieces = 0, total;
+        if (k < r) {
+            const int32_t seg = l.order[k];
+            const int64_t len = l.off[seg + 1] - l.off[seg];
+            pieces = grad_pieces(len, piece).count;
+        }
+        const int64_t item = items + block_scan(pieces * per_segment, warps, total);
+        items += total;
+        const int64_t c = cut + block_scan(pieces > 1 ? per_segment : 0, warps, total);
+        cut += total;
+        const int64_t slot = slots + block_scan(pieces > 1 ? pieces * per_segment : 0, warps, total);
+        slots += total;
+        if (k < r) {
+            l.item_off[k] = item;
+            l.cut_off[k] = c;
+            l.slot_off[k] = slot;
         }
     }
-    const int64_t even = units / ctas + (all / ctas + 2) * kTileCost + kJoinCost;
-    if (most > even) *l.mode = 1;
-}
-
-// Rows past the last segment: da = 0.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    k_zero_rows(T *__restrict__ da, const int64_t *__restrict__ off, int64_t r, int64_t n,
-                int64_t d1) {
-    for (int64_t i = off[r] * d1 + blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n * d1;
-         i += (int64_t)gridDim.x * blockDim.x)
-        da[i] = from_acc<T>(0);
+    if (threadIdx.x == 0) {
+        l.item_off[r] = items;
+        l.cut_off[r] = cut;
+        l.slot_off[r] = slots;
+        l.head[kHeadItems] = items + da_items;
+        l.head[kHeadDbItems] = items;
+        l.head[kHeadPiece] = piece;
+        l.head[kHeadCut] = cut;
+        l.head[kHeadNext] = t.ctas;  // the first items are the CTAs' own numbers
+    }
 }
 
 // 64 x 64 outputs a block of 256 threads, 4 x 4 a thread, over a shared strip
@@ -238,16 +265,23 @@ int simt(const void *g, const void *a, const void *b, const int64_t *off, int64_
 }
 
 GradLayout grad_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype) {
+    const GradTiles t = gmm_grad_tiles(n, d1, r, d2);
     Carver c(ws);
     GradLayout l;
     l.off = c.take<int64_t>((size_t)r + 1);
-    l.tile_off = c.take<int64_t>((size_t)r + 1);
-    l.unit_off = c.take<int64_t>((size_t)r + 1);
-    l.mode = c.take<int64_t>(1);
-    // two partial tiles a CTA: the one it begins with and the one it ends with
-    l.partial = dtype == BGL_BF16
-                    ? c.take<float>((size_t)gmm_grad_tiles(n, d1, r, d2).ctas * 2 * kGradTile * kGradTile)
-                    : nullptr;
+    l.row_off = c.take<int64_t>((size_t)r + 1);
+    l.order = c.take<int32_t>((size_t)r);
+    l.item_off = c.take<int64_t>((size_t)r + 1);
+    l.cut_off = c.take<int64_t>((size_t)r + 1);
+    l.slot_off = c.take<int64_t>((size_t)r + 1);
+    l.head = c.take<int64_t>(kHead);
+    l.partial = nullptr;
+    if (dtype == BGL_BF16) {
+        // no tile is cut below 8 slices
+        int64_t slots = (int64_t)t.ctas * kGradSlots;
+        const int64_t most = t.tiles1 * t.tiles2 * 2 * (n / kGradSlice) / 8;
+        l.partial = c.take<float>((size_t)(slots < most ? slots : most) * kGradTile * kGradTile);
+    }
     l.bytes = c.used + 256;
     return l;
 }
@@ -282,33 +316,15 @@ int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, cons
         return fail(BGL_E_WORKSPACE, "%s: workspace too small", who);
     cudaStream_t s = as_stream(stream);
     const bool want_da = da && n && d1, want_db = db && r && d1 && d2;
-    const bool da_tc = want_da && dtype == BGL_BF16 && r && d2 &&
-                       gmm_tensor_core_supported(d2, d1, dtype) && gmm_tensor_core_fits(n, r, d1) &&
-                       aligned(grad, 16) && aligned(b, 16) && aligned(da, 16);
-    const bool db_tc = want_db && gmm_grad_tc_supported(grad, a, db, n, d1, r, d2, dtype);
     const GradTiles t = gmm_grad_tiles(n, d1, r, d2);
-    k_grad_schedule<<<1, 1024, 0, s>>>(seglen, r, n, t.per_segment, db_tc ? t.ctas : 0, l);
+    const bool tc = r && gmm_grad_tc_supported(grad, a, b, want_da ? da : nullptr,
+                                               want_db ? db : nullptr, n, d1, r, d2, dtype);
+    k_grad_schedule<<<1, 1024, 0, s>>>(seglen, r, n, t, (d2 + kGradSlice - 1) / kGradSlice,
+                                       tc && want_da, tc && want_db, l);
     BGL_LAUNCH_CHECK();
-    if (da_tc) {
-        const int64_t blocks = (n * d1 + 255) / 256, cap = (int64_t)num_sms() * 8;
-        k_zero_rows<__nv_bfloat16><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, s>>>(
-            (__nv_bfloat16 *)da, l.off, r, n, d1);
-        BGL_LAUNCH_CHECK();
-        // b[r] is (d1, d2): rows of the product's columns, already K-major
-        GmmLayout g = {};
-        g.seg_off = l.off;
-        g.tile_off = l.tile_off;
-        g.tc_b = const_cast<void *>(b);
-        const int rc = gmm_tensor_core(grad, nullptr, da, g, n, d2, r, d1, dtype, s);
-        if (rc) return rc;
-    }
-    if (db_tc) {
-        const int rc = gmm_grad_tensor_core(grad, a, db, l, t, n, d1, r, d2, s);
-        if (rc) return rc;
-    }
-    if (da_tc || !want_da) da = nullptr;
-    if (db_tc || !want_db) db = nullptr;
-    if (!da && !db) return BGL_OK;
+    if (!want_da) da = nullptr;
+    if (!want_db) db = nullptr;
+    if (tc) return gmm_grad_tensor_core(grad, a, b, da, db, l, t, n, d1, r, d2, s);
     if (dtype == BGL_F64) return simt<double>(grad, a, b, l.off, n, d1, r, d2, da, db, s);
     if (dtype == BGL_F32) return simt<float>(grad, a, b, l.off, n, d1, r, d2, da, db, s);
     return simt<__nv_bfloat16>(grad, a, b, l.off, n, d1, r, d2, da, db, s);

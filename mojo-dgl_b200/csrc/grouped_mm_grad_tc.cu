@@ -1,23 +1,27 @@
-// tcgen05 kernel for the weight gradient of segment_mm in bfloat16:
-// db[r] = a[rows of r]^T @ grad[rows of r], float32 sums.
+// tcgen05 kernel for the gradients of segment_mm in bfloat16, float32 sums:
 //
-// The sum runs over rows, so both operands are read as they lie in memory, 64
-// rows x 64 columns a TMA box, and are M- and N-major for the tensor cores (no
-// transposed copies).  A CTA owns a 256 x 256 tile of a segment's block: two
-// 128 x 256 float32 accumulators fill the tensor memory, and each 64-row slice
-// of 32 KB + 32 KB feeds 2 x 4 MMAs, so a loaded byte meets twice the products
-// of a 128 x 256 tile.  Warp 0 issues the loads into a three-slice ring, warp 1
-// the MMAs, warps 2-9 write finished tiles out (through a swizzled staging box
-// and TMA stores, clipped to the segment's block by the 3-D tensor map).
+//   da[i] = grad[i] @ b[r]^T                  (K = d2: both operands K-major)
+//   db[r] = a[rows of r]^T @ grad[rows of r]  (K = rows: both M/N-major)
 //
-// A slice's rows beyond the segment belong to the next one: the MMA warp writes
-// zeros over those that share a 16-row MMA step with the segment's last rows
-// (in both operands, so that inf and NaN of a neighbour do not get in) and
-// leaves out the steps behind.
+// Every operand is read as it lies in memory, 64 rows x 64 columns a TMA box;
+// a box serves as K-major rows or as M/N-major columns, so the two products
+// differ only in coordinates and descriptors, and no transposed copy is made.
+// A CTA works on one 256 x 256 tile at a time: two 128 x 256 float32
+// accumulators fill the tensor memory, and each K slice of 64 (32 KB + 32 KB)
+// feeds 2 x 4 MMAs, so a loaded byte meets 4/3 of the products of a 128 x 256
+// tile: what bounds wide blocks is the rate at which L2 hands out tiles.
 //
-// Units (one slice of one tile) are handed out as whole tiles, or split evenly
-// over the CTAs (GradLayout::mode): a tile cut between CTAs then goes to float32
-// partial tiles, which k_grad_join adds in order -- the same bits on every run.
+// One persistent launch holds both products.  Warp 10 takes the next item (an
+// atomic counter; which CTA does what does not change any result) and
+// publishes it through a four-deep queue, warp 0 issues the loads into a
+// three-slice ring, warp 1 the MMAs, warps 2-9 write finished tiles out
+// (through a swizzled staging box and TMA stores).
+//
+// A db slice's rows beyond the segment belong to the next one: the MMA warp
+// writes zeros over those that share a 16-row MMA step with the segment's last
+// rows (in both operands, so that inf and NaN of a neighbour do not get in) and
+// leaves out the steps behind.  Pieces of a cut db tile go to float32 partial
+// tiles, which k_grad_finish adds in order: the same bits on every run.
 //
 // Every mbarrier wait is bounded, with the abort protocol of grouped_mm_tc.cu.
 #include "grouped_mm.cuh"
@@ -28,76 +32,81 @@ namespace {
 
 constexpr int kStages = 3;
 constexpr int kBox = kGradSlice * 128;        // 64 rows x 64 columns of bf16
-constexpr int kStageBytes = 8 * kBox;         // 4 boxes of a, 4 of grad
+constexpr int kStageBytes = 8 * kBox;         // 4 boxes of each operand
 constexpr int kEpiWarps = 8;                  // two a TMEM lane quarter, one for each half
-constexpr int kWarpLoad = 0, kWarpMma = 1, kWarpEpi0 = 2;
-constexpr int kThreads = 32 * (kWarpEpi0 + kEpiWarps);
+constexpr int kQueue = 4;
+constexpr int kWarpLoad = 0, kWarpMma = 1, kWarpEpi0 = 2, kWarpNext = kWarpEpi0 + kEpiWarps;
+constexpr int kThreads = 32 * (kWarpNext + 1);
 constexpr int kPartial = kGradTile * kGradTile;  // values of a partial tile
-constexpr size_t kSmem = 1024 + kStages * (size_t)kStageBytes + kEpiWarps * 4096 + 8 * (2 * kStages + 4) + 16;
 
 struct GradArgs {
-    const int64_t *off, *unit_off, *mode;
+    const int64_t *off, *row_off, *item_off, *cut_off, *slot_off;
+    const int32_t *order;
+    int64_t *head;
     float *partial;
-    int64_t r, per_segment;
-    int32_t tiles_n, d1, d2;
+    __nv_bfloat16 *da, *db;
+    int64_t r, n;
+    int32_t tiles1, tiles2, d1, d2;
 };
 
-// What a CTA does to one tile: rows [row0, row0 + rows) of segment seg, the
-// tile at (i0, j0) of the segment's block; `slot` is the partial tile it goes
-// to, -1 where it is the whole sum.
-struct Piece {
-    int64_t seg, row0, rows;
-    int32_t i0, j0;
-    int64_t slot;
-    bool lead;  // holds the tile's first rows
+// One item.  da: rows [row0, row0 + rows) of segment seg, columns from j0 on.
+// db: the sum over those rows for the tile at (i0, j0) of the segment's block;
+// `slot` is the partial tile it goes to, -1 where it is the whole sum.
+struct Item {
+    int32_t kind;  // 0: none left, 1: da, 2: db
+    int32_t seg, row0, rows, i0, j0, slot;
 };
+constexpr int kDa = 1, kDb = 2;
+constexpr size_t kSmem = 1024 + kStages * (size_t)kStageBytes + kEpiWarps * 4096 +
+                         8 * (2 * kStages + 2 * kQueue + 4) + kQueue * sizeof(Item) + 16;
 
-// Walks a CTA's pieces; every role of the CTA sees the same ones.
-struct Walk {
-    int64_t at, end;  // tiles (whole) or units (split)
-    bool split;
-
-    __device__ __forceinline__ Walk(const GradArgs &p, int64_t cta, int64_t ctas) {
-        split = *p.mode != 0;
-        const int64_t units = p.unit_off[p.r];
-        at = split ? units * cta / ctas : cta;
-        end = split ? units * (cta + 1) / ctas : p.r * p.per_segment;
+// Last i in [0, n) with first[i] <= at, by the whole warp (33 ways a step).
+__device__ __forceinline__ int64_t warp_search(const int64_t *first, int64_t n, int64_t at) {
+    const int lane = threadIdx.x & 31;
+    int64_t lo = 0, hi = n;  // first[lo] <= at < first[hi]
+    while (hi - lo > 1) {
+        const int64_t step = (hi - lo + 32) / 33, i = lo + (lane + 1) * step;
+        const unsigned below = __ballot_sync(0xffffffffu, i < hi && first[i < hi ? i : lo] <= at);
+        const int64_t base = lo + (int64_t)__popc(below) * step;
+        if (base + step < hi) hi = base + step;
+        lo = base;
     }
+    return lo;
+}
 
-    __device__ __forceinline__ bool next(const GradArgs &p, int64_t cta, int64_t ctas, Piece &q) {
-        if (at >= end) return false;
-        int64_t tile, k = 0, take;
-        if (split) {
-            int64_t lo = 0, hi = p.r - 1;  // last segment whose first unit is <= at
-            while (lo < hi) {
-                const int64_t mid = (lo + hi + 1) >> 1;
-                if (p.unit_off[mid] <= at) lo = mid; else hi = mid - 1;
-            }
-            q.seg = lo;
-            const int64_t slices = (p.unit_off[lo + 1] - p.unit_off[lo]) / p.per_segment;
-            const int64_t in = at - p.unit_off[lo];
-            tile = in / slices;
-            k = in % slices;
-            take = slices - k < end - at ? slices - k : end - at;
-            q.lead = k == 0;
-            q.slot = q.lead && take == slices ? -1 : 2 * cta + (q.lead ? 1 : 0);
-            at += take;
-        } else {
-            q.seg = at / p.per_segment;
-            tile = at % p.per_segment;
-            take = INT32_MAX;
-            q.lead = true;
-            q.slot = -1;
-            at += ctas;
-        }
-        const int64_t first = p.off[q.seg] + k * kGradSlice, last = p.off[q.seg + 1];
-        q.row0 = first;
-        q.rows = last - first < take * kGradSlice ? last - first : take * kGradSlice;
-        q.i0 = (int32_t)(tile / p.tiles_n) * kGradTile;
-        q.j0 = (int32_t)(tile % p.tiles_n) * kGradTile;
-        return true;
+// Item number `at`, on every lane of the warp.
+__device__ __forceinline__ Item item_at(const GradArgs &p, int64_t at) {
+    Item q = {};
+    const int64_t db_items = p.head[kHeadDbItems];
+    if (at >= p.head[kHeadItems]) return q;
+    if (at < db_items) {
+        const int64_t k = warp_search(p.item_off, p.r, at);
+        q.kind = kDb;
+        q.seg = p.order[k];
+        const int64_t first = p.off[q.seg], len = p.off[q.seg + 1] - first;
+        const GradPieces cut = grad_pieces(len, p.head[kHeadPiece]);
+        const int64_t in = at - p.item_off[k], per = (int64_t)p.tiles1 * p.tiles2;
+        // the tiles of one piece are neighbours: they read the same rows
+        const int64_t piece = in / per, tile = in % per;
+        q.i0 = (int32_t)(tile / p.tiles2) * kGradTile;
+        q.j0 = (int32_t)(tile % p.tiles2) * kGradTile;
+        const int64_t skip = piece * cut.slices * kGradSlice, most = cut.slices * kGradSlice;
+        q.row0 = (int32_t)(first + skip);
+        q.rows = (int32_t)(len - skip < most ? len - skip : most);
+        q.slot = cut.count > 1 ? (int32_t)(p.slot_off[k] + tile * cut.count + piece) : -1;
+    } else {
+        const int64_t in = at - db_items, tile = in / p.tiles1;
+        q.kind = kDa;
+        q.seg = (int32_t)warp_search(p.row_off, p.r, tile);
+        const int64_t first = p.off[q.seg] + (tile - p.row_off[q.seg]) * kGradTile;
+        const int64_t left = p.off[q.seg + 1] - first;
+        q.row0 = (int32_t)first;
+        q.rows = (int32_t)(left < kGradTile ? left : kGradTile);
+        q.j0 = (int32_t)(in % p.tiles1) * kGradTile;
+        q.slot = -1;
     }
-};
+    return q;
+}
 
 // SWIZZLE_128B descriptor of an M- or N-major operand: 64-element runs of 128
 // bytes, one a row of K; 8-row groups 1024 bytes apart (SBO), the next 64
@@ -107,10 +116,13 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// fp32 accumulator, bf16 operands, both M/N-major, M = 128.
+// Instruction descriptors: fp32 accumulator, bf16 operands, M = 128, both
+// operands K-major or both M/N-major.
+__device__ __forceinline__ uint32_t k_instr(int n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
 __device__ __forceinline__ uint32_t mn_instr(int n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    return k_instr(n) | (1u << 15) | (1u << 16);
 }
 
 // Lane 0 waits for the whole warp.
@@ -132,8 +144,27 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void 
         : "memory");
 }
 
+// How the roles see an item: the boxes of each operand that are loaded, and the
+// K slices.
+struct Shape {
+    int boxes_m, boxes_n, halves, slices, n;
+};
+__device__ __forceinline__ Shape shape_of(const GradArgs &p, const Item &q) {
+    Shape s;
+    const int m = q.kind == kDa ? q.rows : p.d1 - q.i0;
+    const int n = q.kind == kDa ? p.d1 - q.j0 : p.d2 - q.j0;
+    const int k = q.kind == kDa ? p.d2 : q.rows;
+    s.boxes_m = min(4, (m + 63) / 64);
+    s.boxes_n = min(4, (n + 63) / 64);
+    s.halves = m > 128 ? 2 : 1;
+    s.slices = (k + kGradSlice - 1) / kGradSlice;
+    s.n = min(kGradTile, (n + 15) / 16 * 16);
+    return s;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     k_grad_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_g,
+              const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_da,
               const __grid_constant__ CUtensorMap map_db, const GradArgs args) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -142,16 +173,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint4 *staging = reinterpret_cast<uint4 *>(ring + kStages * kStageBytes);
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + kStages * kStageBytes + kEpiWarps * 4096);
     uint64_t *empty = full + kStages;
-    uint64_t *acc_full = empty + kStages;
+    uint64_t *next_full = empty + kStages;      // [kQueue] an item has been published
+    uint64_t *next_empty = next_full + kQueue;  // [kQueue] every role has read it
+    uint64_t *acc_full = next_empty + kQueue;
     uint64_t *acc_empty = acc_full + 1;  // [2]: a half of the accumulators has been read
     uint64_t *mma_done = acc_empty + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
+    Item *queue = reinterpret_cast<Item *>(mma_done + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(queue + kQueue);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kQueue; ++s) {
+            mbar_init(&next_full[s], 1);
+            mbar_init(&next_empty[s], 2 + kEpiWarps);
         }
         mbar_init(acc_full, 1);
         mbar_init(&acc_empty[0], kEpiWarps / 2);
@@ -170,71 +208,112 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    const int64_t cta = blockIdx.x, ctas = gridDim.x;
-    Walk walk(args, cta, ctas);
-    Piece q;
 
-    if (warp == kWarpLoad) {
-        if (lane == 0) {
-            int64_t it = 0;
-            bool ok = true;
-            while (ok && walk.next(args, cta, ctas, q)) {
-                // boxes that lie inside the block; the others' columns are not used
-                const int na = min(4, (args.d1 - q.i0 + 63) / 64), ng = min(4, (args.d2 - q.j0 + 63) / 64);
-                for (int64_t k = 0; k < q.rows; k += kGradSlice, ++it) {
-                    const int s = (int)(it % kStages);
-                    if (it >= kStages &&
-                        !(ok = mbar_wait(&empty[s], (uint32_t)((it / kStages) - 1) & 1, 1, abort)))
-                        break;
-                    unsigned char *stage = ring + s * kStageBytes;
-                    mbar_arrive_expect_tx(&full[s], (uint32_t)(na + ng) * kBox);
-                    const int32_t row = (int32_t)(q.row0 + k);
-                    for (int b = 0; b < na; ++b)
-                        tma_load_2d(stage + b * kBox, &map_a, &full[s], q.i0 + 64 * b, row);
-                    for (int b = 0; b < ng; ++b)
-                        tma_load_2d(stage + (4 + b) * kBox, &map_g, &full[s], q.j0 + 64 * b, row);
-                }
+    // Item t of this CTA, for a whole warp: false when none is left.
+    auto take = [&](int64_t t, Item &q) {
+        const int s = (int)(t % kQueue);
+        if (!warp_wait(&next_full[s], (uint32_t)(t / kQueue) & 1, 7, abort)) return false;
+        q = queue[s];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&next_empty[s]);
+        return q.kind != 0;
+    };
+
+    if (warp == kWarpNext) {
+        int64_t at = blockIdx.x;
+        for (int64_t t = 0;; ++t) {
+            const int s = (int)(t % kQueue);
+            if (t >= kQueue && !warp_wait(&next_empty[s], (uint32_t)(t / kQueue - 1) & 1, 8, abort)) break;
+            const Item q = item_at(args, at);
+            if (lane == 0) {
+                queue[s] = q;
+                mbar_arrive(&next_full[s]);
             }
-            // the last issued loads (at most one per stage) have landed before exit
-            for (int64_t j = (it > kStages ? it - kStages : 0); j < it; ++j)
-                mbar_wait(&full[j % kStages], (uint32_t)(j / kStages) & 1, 2, nullptr);
+            if (!q.kind) break;
+            if (lane == 0)
+                at = (int64_t)atomicAdd(reinterpret_cast<unsigned long long *>(&args.head[kHeadNext]), 1ull);
+            at = __shfl_sync(0xffffffffu, at, 0);
         }
-    } else if (warp == kWarpMma) {
-        int64_t it = 0, t = 0;
+    } else if (warp == kWarpLoad) {
+        int64_t it = 0;
         bool ok = true;
-        for (; ok && walk.next(args, cta, ctas, q); ++t) {
-            const int halves = args.d1 - q.i0 > 128 ? 2 : 1;
-            const int na = min(4, (args.d1 - q.i0 + 63) / 64), ng = min(4, (args.d2 - q.j0 + 63) / 64);
-            const uint32_t idesc = mn_instr(min(256, (args.d2 - q.j0 + 15) / 16 * 16));
+        Item q;
+        for (int64_t t = 0; ok && take(t, q); ++t) {
+            const Shape sh = shape_of(args, q);
+            for (int k = 0; k < sh.slices; ++k, ++it) {
+                const int s = (int)(it % kStages);
+                if (it >= kStages &&
+                    !(ok = warp_wait(&empty[s], (uint32_t)((it / kStages) - 1) & 1, 1, abort)))
+                    break;
+                if (lane == 0) {
+                    unsigned char *m = ring + s * kStageBytes, *n = m + 4 * kBox;
+                    mbar_arrive_expect_tx(&full[s], (uint32_t)(sh.boxes_m + sh.boxes_n) * kBox);
+                    if (q.kind == kDa) {
+                        const int32_t row = (int32_t)(q.seg * (int64_t)args.d1) + q.j0;
+                        for (int b = 0; b < sh.boxes_m; ++b)
+                            tma_load_2d(m + b * kBox, &map_g, &full[s], 64 * k, q.row0 + 64 * b);
+                        for (int b = 0; b < sh.boxes_n; ++b)
+                            tma_load_2d(n + b * kBox, &map_b, &full[s], 64 * k, row + 64 * b);
+                    } else {
+                        const int32_t row = q.row0 + kGradSlice * k;
+                        for (int b = 0; b < sh.boxes_m; ++b)
+                            tma_load_2d(m + b * kBox, &map_a, &full[s], q.i0 + 64 * b, row);
+                        for (int b = 0; b < sh.boxes_n; ++b)
+                            tma_load_2d(n + b * kBox, &map_g, &full[s], q.j0 + 64 * b, row);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        // the last issued loads (at most one per stage) have landed before exit
+        for (int64_t j = (it > kStages ? it - kStages : 0); j < it; ++j)
+            mbar_wait(&full[j % kStages], (uint32_t)(j / kStages) & 1, 2, nullptr);
+        __syncwarp();
+    } else if (warp == kWarpMma) {
+        int64_t it = 0;
+        bool ok = true;
+        Item q;
+        for (int64_t t = 0; ok && take(t, q); ++t) {
+            const Shape sh = shape_of(args, q);
+            const uint32_t idesc = q.kind == kDa ? k_instr(sh.n) : mn_instr(sh.n);
             bool waited = t == 0;  // the epilogue has read the previous tile
-            for (int64_t k = 0; k < q.rows; k += kGradSlice, ++it) {
+            for (int k = 0; k < sh.slices; ++k, ++it) {
                 const int s = (int)(it % kStages);
                 if (!(ok = warp_wait(&full[s], (uint32_t)(it / kStages) & 1, 3, abort))) break;
-                unsigned char *stage = ring + s * kStageBytes;
-                const int rows = q.rows - k < kGradSlice ? (int)(q.rows - k) : kGradSlice;
-                const int steps = (rows + 15) / 16;
-                if (rows & 15) {
-                    // 8 pieces of 16 bytes a row and box
-                    const int zero = (steps * 16 - rows) * 8;
-                    for (int b = 0; b < 8; ++b) {
-                        if (b < 4 ? b >= na : b - 4 >= ng) continue;
-                        uint4 *p = reinterpret_cast<uint4 *>(stage + b * kBox + rows * 128);
-                        for (int i = lane; i < zero; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+                unsigned char *m = ring + s * kStageBytes, *n = m + 4 * kBox;
+                int steps = kGradSlice / 16;
+                if (q.kind == kDb && q.rows - k * kGradSlice < kGradSlice) {
+                    const int rows = q.rows - k * kGradSlice;
+                    steps = (rows + 15) / 16;
+                    const int zero = (steps * 16 - rows) * 8;  // 16-byte pieces of a box
+                    if (zero) {
+                        for (int b = 0; b < 8; ++b) {
+                            if (b < 4 ? b >= sh.boxes_m : b - 4 >= sh.boxes_n) continue;
+                            uint4 *p = reinterpret_cast<uint4 *>(m + b * kBox + rows * 128);
+                            for (int i = lane; i < zero; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
                     }
-                    fence_proxy_async_smem();
-                    __syncwarp();
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int h = 0; h < halves; ++h) {
-                    if (!waited && !(ok = warp_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort))) break;
-                    if (!waited) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int h = 0; h < sh.halves; ++h) {
+                    if (!waited) {
+                        if (!(ok = warp_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
                     if (lane == 0) {
-                        const uint64_t ad = mn_desc(smem_u32(stage + h * 2 * kBox));
-                        const uint64_t gd = mn_desc(smem_u32(stage + 4 * kBox));
-                        for (int kk = 0; kk < steps; ++kk)  // 16 rows: 2048 bytes further on
-                            mma<true>(tmem + 256u * h, ad + kk * 128, gd + kk * 128, idesc,
+                        // a half is 128 rows of K runs, or two boxes of 64 columns
+                        const uint32_t am = smem_u32(m + h * 2 * kBox), an = smem_u32(n);
+                        const bool da = q.kind == kDa;
+                        const uint64_t ad = da ? smem_desc(am) : mn_desc(am);
+                        const uint64_t bd = da ? smem_desc(an) : mn_desc(an);
+                        const int step = da ? 2 : 128;  // 16 of K: 32 bytes, or 16 rows of 128
+                        for (int kk = 0; kk < steps; ++kk)
+                            mma<true>(tmem + 256u * h, ad + kk * step, bd + kk * step, idesc,
                                       (k | kk) != 0);
                     }
+                    __syncwarp();
                 }
                 if (!ok) break;
                 waited = true;
@@ -244,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // a half that this tile does not write (both, for a tile without
             // rows) takes its turn as well: acc_full moves on by one tile only
             // when every epilogue warp has seen the one before
-            for (int h = waited ? halves : 0; ok && t > 0 && h < 2; ++h)
+            for (int h = waited ? sh.halves : 0; ok && t > 0 && h < 2; ++h)
                 ok = warp_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort);
             if (!ok) break;
             if (lane == 0) mma_commit(acc_full);
@@ -259,52 +338,69 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // warp w reads TMEM lanes [32 (w % 4), 32 (w % 4) + 32) of one half
         const int quarter = warp & 3, half = (warp - kWarpEpi0) >> 2;
+        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + 256u * half;
         uint4 *stg = staging + (warp - kWarpEpi0) * 256;
-        for (int64_t t = 0; walk.next(args, cta, ctas, q); ++t) {
+        const int line = half * 128 + quarter * 32;  // first row of the tile here
+        Item q;
+        for (int64_t t = 0; take(t, q); ++t) {
             if (!warp_wait(acc_full, (uint32_t)t & 1, 4, abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int32_t i0 = q.i0 + half * 128 + quarter * 32;
-            const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + 256u * half;
-            const bool none = q.rows <= 0;
-            if (i0 < args.d1) {
-                for (int c = 0; c < 256 && q.j0 + c < args.d2; c += 64) {
-                    uint32_t v[64];
-                    if (none) {
+            const bool da = q.kind == kDa;
+            const int rows = (da ? q.rows : args.d1 - q.i0) - line;  // those that exist
+            const int cols = (da ? args.d1 : args.d2) - q.j0;
+            const bool none = !da && q.rows <= 0;
+            for (int c = 0; rows > 0 && c < kGradTile && c < cols; c += 64) {
+                uint32_t v[64];
+                if (none) {
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) v[i] = 0;
-                    } else {
+                    for (int i = 0; i < 64; ++i) v[i] = 0;
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tmem_ld16(taddr + (uint32_t)(c + 16 * i),
-                                      *reinterpret_cast<uint32_t(*)[16]>(&v[16 * i]));
-                        tmem_wait_ld();
+                    for (int i = 0; i < 4; ++i)
+                        tmem_ld16(taddr + (uint32_t)(c + 16 * i),
+                                  *reinterpret_cast<uint32_t(*)[16]>(&v[16 * i]));
+                    tmem_wait_ld();
+                }
+                if (q.slot >= 0) {
+                    // [half][16-byte column group][row of the half]: whole lines a warp
+                    uint4 *dst = reinterpret_cast<uint4 *>(args.partial + (int64_t)q.slot * kPartial) +
+                                 (half * 64 + c / 4) * 128 + quarter * 32 + lane;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        dst[i * 128] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    continue;
+                }
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]),
+                                                                  __uint_as_float(v[8 * j + 2 * i + 1]));
+                        o[i] = *reinterpret_cast<uint32_t *>(&h2);
                     }
-                    if (q.slot >= 0) {
-                        // [half][16-byte column group][row of the half]: whole lines a warp
-                        uint4 *dst = reinterpret_cast<uint4 *>(args.partial + q.slot * kPartial) +
-                                     (half * 64 + c / 4) * 128 + quarter * 32 + lane;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            dst[i * 128] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        continue;
-                    }
-                    if (lane == 0) bulk_wait_read<0>();
+                    stg[lane * 8 + (j ^ (lane & 7))] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                if (da && rows < 32) {
+                    // the segment's last rows: the next segment's must not be written
                     __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t o[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]),
-                                                                      __uint_as_float(v[8 * j + 2 * i + 1]));
-                            o[i] = *reinterpret_cast<uint32_t *>(&h2);
-                        }
-                        stg[lane * 8 + (j ^ (lane & 7))] = make_uint4(o[0], o[1], o[2], o[3]);
+                    for (int i = lane; i < rows * 8; i += 32) {
+                        const int row = i >> 3, j = i & 7, col = q.j0 + c + j * 8;
+                        if (col < args.d1)
+                            *reinterpret_cast<uint4 *>(args.da + ((int64_t)q.row0 + line + row) * args.d1 + col) =
+                                stg[row * 8 + (j ^ (row & 7))];
                     }
+                    __syncwarp();
+                } else {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(&map_db, stg, q.j0 + c, i0, (int32_t)q.seg);
+                        if (da)
+                            tma_store_2d(&map_da, stg, q.j0 + c, q.row0 + line);
+                        else  // clipped to the segment's block
+                            tma_store_3d(&map_db, stg, q.j0 + c, q.i0 + line, q.seg);
                         bulk_commit();
                     }
                 }
@@ -314,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&acc_empty[half]);
         }
         if (lane == 0) bulk_wait_all();
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -323,56 +420,55 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Adds the partial tiles of the tiles that were cut: block (c, part) takes the
-// tile that CTA c began and did not finish, 16 columns a thread.
-__global__ void __launch_bounds__(256)
-    k_grad_join(const GradArgs args, int64_t ctas, __nv_bfloat16 *__restrict__ db) {
-    if (*args.mode == 0) return;
-    Walk walk(args, blockIdx.x, ctas);
-    Piece q, last;
-    last.slot = -1;
-    while (walk.next(args, blockIdx.x, ctas, q)) last = q;
-    if (last.slot < 0 || !last.lead) return;
-    // the CTAs that hold the rest: up to the one that ends with the segment's rows
-    const int64_t seg_end = args.off[last.seg + 1];
-    int64_t row = last.row0 + last.rows, more = blockIdx.x;
-    while (row < seg_end && more + 1 < ctas) {
-        Walk other(args, ++more, ctas);
-        if (other.next(args, more, ctas, q)) row = q.row0 + q.rows;
+// Adds the pieces of db's cut tiles, 16 columns a thread, and zeroes the rows of
+// da past the last segment.
+__global__ void __launch_bounds__(256) k_grad_finish(const GradArgs args) {
+    if (args.da) {
+        const int64_t first = args.off[args.r] * args.d1 / 8, end = args.n * args.d1 / 8;
+        const int64_t block = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+        uint4 *da = reinterpret_cast<uint4 *>(args.da);  // d1 is a multiple of 8
+        for (int64_t i = first + block * 256 + threadIdx.x; i < end;
+             i += (int64_t)gridDim.x * gridDim.y * 256)
+            da[i] = make_uint4(0, 0, 0, 0);
     }
-    const int idx = blockIdx.y * 256 + threadIdx.x;  // half, 16 groups of 16 columns, 128 rows
-    const int line = idx & 127, group = (idx >> 7) & 15, half = idx >> 11;
-    const int32_t i = last.i0 + half * 128 + line, j = last.j0 + group * 16;
-    if (i >= args.d1 || j >= args.d2) return;
-    float4 sum[4];
-    for (int64_t c = blockIdx.x; c <= more; ++c) {
-        const Walk other(args, c, ctas);
-        if (other.at >= other.end) continue;  // a CTA without units
-        const int64_t slot = c == blockIdx.x ? last.slot : 2 * c;
-        const float4 *src = reinterpret_cast<const float4 *>(args.partial + slot * kPartial) +
+    if (!args.db) return;
+    const int64_t cuts = args.head[kHeadCut];
+    for (int64_t cut = blockIdx.x; cut < cuts; cut += gridDim.x) {
+        const int64_t k = warp_search(args.cut_off, args.r, cut);
+        const int32_t seg = args.order[k];
+        const int64_t tile = cut - args.cut_off[k];
+        const int64_t count = grad_pieces(args.off[seg + 1] - args.off[seg], args.head[kHeadPiece]).count;
+        const int idx = blockIdx.y * 256 + threadIdx.x;  // half, 16 groups of 16 columns, 128 rows
+        const int line = idx & 127, group = (idx >> 7) & 15, half = idx >> 11;
+        const int32_t i = (int32_t)(tile / args.tiles2) * kGradTile + half * 128 + line;
+        const int32_t j = (int32_t)(tile % args.tiles2) * kGradTile + group * 16;
+        if (i >= args.d1 || j >= args.d2) continue;
+        const float4 *src = reinterpret_cast<const float4 *>(
+                                args.partial + (args.slot_off[k] + tile * count) * kPartial) +
                             (half * 64 + group * 4) * 128 + line;
+        float4 sum[4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const float4 x = src[v * 128];
-            if (c == blockIdx.x) {
-                sum[v] = x;
-            } else {
+        for (int v = 0; v < 4; ++v) sum[v] = src[v * 128];
+        for (int64_t p = 1; p < count; ++p) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float4 x = src[p * (kPartial / 4) + v * 128];
                 sum[v].x += x.x;
                 sum[v].y += x.y;
                 sum[v].z += x.z;
                 sum[v].w += x.w;
             }
         }
-    }
-    __nv_bfloat16 *dst = db + (last.seg * args.d1 + i) * (int64_t)args.d2 + j;
+        __nv_bfloat16 *dst = args.db + (seg * (int64_t)args.d1 + i) * args.d2 + j;
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {  // d2 is a multiple of 8
-        if (j + 8 * v >= args.d2) break;
-        __nv_bfloat162 o[4] = {__floats2bfloat162_rn(sum[2 * v].x, sum[2 * v].y),
-                               __floats2bfloat162_rn(sum[2 * v].z, sum[2 * v].w),
-                               __floats2bfloat162_rn(sum[2 * v + 1].x, sum[2 * v + 1].y),
-                               __floats2bfloat162_rn(sum[2 * v + 1].z, sum[2 * v + 1].w)};
-        *reinterpret_cast<uint4 *>(dst + 8 * v) = *reinterpret_cast<uint4 *>(o);
+        for (int v = 0; v < 2; ++v) {  // d2 is a multiple of 8
+            if (j + 8 * v >= args.d2) break;
+            __nv_bfloat162 o[4] = {__floats2bfloat162_rn(sum[2 * v].x, sum[2 * v].y),
+                                   __floats2bfloat162_rn(sum[2 * v].z, sum[2 * v].w),
+                                   __floats2bfloat162_rn(sum[2 * v + 1].x, sum[2 * v + 1].y),
+                                   __floats2bfloat162_rn(sum[2 * v + 1].z, sum[2 * v + 1].w)};
+            *reinterpret_cast<uint4 *>(dst + 8 * v) = *reinterpret_cast<uint4 *>(o);
+        }
     }
 }
 
@@ -395,46 +491,60 @@ int bf16_map(CUtensorMap *map, const void *ptr, int rank, const int64_t *dims, u
 
 }  // namespace
 
-// TMA wants 16-byte aligned bases and row strides.
-bool gmm_grad_tc_supported(const void *grad, const void *a, const void *db, int64_t n, int64_t d1,
-                           int64_t r, int64_t d2, int dtype) {
-    return dtype == BGL_BF16 && n > 0 && d1 > 0 && d2 > 0 && d1 % 8 == 0 && d2 % 8 == 0 &&
-           d1 * d2 < (int64_t(1) << 39) && aligned(grad, 16) && aligned(a, 16) && aligned(db, 16);
+// TMA wants 16-byte aligned bases and row strides, and 32-bit row numbers.
+bool gmm_grad_tc_supported(const void *grad, const void *a, const void *b, const void *da,
+                           const void *db, int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype) {
+    return dtype == BGL_BF16 && (da || db) && n > 0 && d1 > 0 && d2 > 0 && d1 % 8 == 0 &&
+           d2 % 8 == 0 && n < (int64_t(1) << 31) - 1024 &&
+           r * d1 < (int64_t(1) << 31) - 1024 &&
+           d1 * d2 < (int64_t(1) << 39) && aligned(grad, 16) && (!da || (aligned(da, 16) && aligned(b, 16))) &&
+           (!db || (aligned(db, 16) && aligned(a, 16)));
 }
 
 GradTiles gmm_grad_tiles(int64_t n, int64_t d1, int64_t r, int64_t d2) {
     GradTiles t;
-    t.tiles_n = (d2 + kGradTile - 1) / kGradTile;
-    t.per_segment = t.tiles_n * ((d1 + kGradTile - 1) / kGradTile);
-    // no more CTAs than there can be units
-    const int64_t units = t.per_segment * (n / kGradSlice + r);
-    t.ctas = (int)(units < num_sms() ? (units > 0 ? units : 1) : num_sms());
+    t.tiles1 = (d1 + kGradTile - 1) / kGradTile;
+    t.tiles2 = (d2 + kGradTile - 1) / kGradTile;
+    // no more CTAs than there can be items: row tiles of da and slices of db
+    const int64_t items = t.tiles1 * (n / kGradTile + r) + t.tiles1 * t.tiles2 * (n / (8 * kGradSlice) + r);
+    t.ctas = (int)(items < num_sms() ? (items > 0 ? items : 1) : num_sms());
     return t;
 }
 
-int gmm_grad_tensor_core(const void *grad, const void *a, void *db, const GradLayout &l,
-                         const GradTiles &t, int64_t n, int64_t d1, int64_t r, int64_t d2,
-                         cudaStream_t s) {
-    CUtensorMap map_a, map_g, map_db;
-    const int64_t dims_a[2] = {d1, n}, dims_g[2] = {d2, n}, dims_db[3] = {d2, d1, r};
-    int rc = bf16_map(&map_a, a, 2, dims_a, kGradSlice);
-    if (!rc) rc = bf16_map(&map_g, grad, 2, dims_g, kGradSlice);
-    if (!rc) rc = bf16_map(&map_db, db, 3, dims_db, 32);
+int gmm_grad_tensor_core(const void *grad, const void *a, const void *b, void *da, void *db,
+                         const GradLayout &l, const GradTiles &t, int64_t n, int64_t d1, int64_t r,
+                         int64_t d2, cudaStream_t s) {
+    CUtensorMap map_a, map_g, map_b, map_da, map_db;
+    const int64_t dims_a[2] = {d1, n}, dims_g[2] = {d2, n}, dims_b[2] = {d2, r * d1},
+                  dims_db[3] = {d2, d1, r};
+    int rc = bf16_map(&map_g, grad, 2, dims_g, kGradSlice);
+    map_a = map_b = map_da = map_db = map_g;  // not read where a gradient is not wanted
+    if (!rc && da) rc = bf16_map(&map_b, b, 2, dims_b, kGradSlice);
+    if (!rc && da) rc = bf16_map(&map_da, da, 2, dims_a, 32);
+    if (!rc && db) rc = bf16_map(&map_a, a, 2, dims_a, kGradSlice);
+    if (!rc && db) rc = bf16_map(&map_db, db, 3, dims_db, 32);
     if (rc) return rc;
     GradArgs args;
     args.off = l.off;
-    args.unit_off = l.unit_off;
-    args.mode = l.mode;
+    args.row_off = l.row_off;
+    args.item_off = l.item_off;
+    args.cut_off = l.cut_off;
+    args.slot_off = l.slot_off;
+    args.order = l.order;
+    args.head = l.head;
     args.partial = l.partial;
+    args.da = static_cast<__nv_bfloat16 *>(da);
+    args.db = static_cast<__nv_bfloat16 *>(db);
     args.r = r;
-    args.per_segment = t.per_segment;
-    args.tiles_n = (int32_t)t.tiles_n;
+    args.n = n;
+    args.tiles1 = (int32_t)t.tiles1;
+    args.tiles2 = (int32_t)t.tiles2;
     args.d1 = (int32_t)d1;
     args.d2 = (int32_t)d2;
     BGL_CUDA(cudaFuncSetAttribute(k_grad_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-    k_grad_tc<<<t.ctas, kThreads, kSmem, s>>>(map_a, map_g, map_db, args);
+    k_grad_tc<<<t.ctas, kThreads, kSmem, s>>>(map_a, map_g, map_b, map_da, map_db, args);
     BGL_LAUNCH_CHECK();
-    k_grad_join<<<dim3((unsigned)t.ctas, 16), 256, 0, s>>>(args, t.ctas, (__nv_bfloat16 *)db);
+    k_grad_finish<<<dim3((unsigned)t.ctas, 16), 256, 0, s>>>(args);
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }

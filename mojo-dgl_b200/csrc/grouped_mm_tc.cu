@@ -472,10 +472,10 @@ int gmm_tensor_core(const void *a, const void *b, void *out, const GmmLayout &l,
                     int64_t d1, int64_t r, int64_t d2, int dtype, cudaStream_t s) {
     const bool bf16 = dtype == BGL_BF16;
     const int64_t elem = bf16 ? 2 : 4;
-    if (!aligned(a, 16) || !aligned(out, 16) || !l.tc_b || !aligned(l.tc_b, 16))
+    if (!aligned(a, 16) || !aligned(out, 16) || !l.tc_b)
         return fail(BGL_E_INVALID, "grouped mm: tensor-core path needs 16-byte aligned operands");
-    // K-major B (b == nullptr: tc_b already holds it)
-    if (b) {
+    // K-major B
+    {
         dim3 grid((unsigned)((d2 + 31) / 32), (unsigned)((d1 + 31) / 32), (unsigned)r);
         if (bf16)
             k_transpose_b<__nv_bfloat16><<<grid, dim3(32, 8), 0, s>>>(
