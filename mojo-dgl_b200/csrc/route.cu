@@ -1,17 +1,33 @@
 // Routing of tokens to experts: scores, selection, weights, and their gradient.
 //
-// A warp per token.  Selection works on order-preserving integer keys of the
-// selection scores, so ties, signed zeros and NaN have one order everywhere:
-// NaN first, then larger scores, equal ones by the lower expert.  Key 0 is an
-// expert that cannot be chosen (a logit or a biased score of -inf, or a group
-// that was not kept).
+// Forward.  Eight lanes work on a token, four tokens a warp.  They load the
+// token's logits in 16-byte pieces, turn them into selection scores and leave
+// those in shared memory, where lane i owns the i-th eighth of the experts and
+// keeps the maximum of every 8 of its scores in registers.  A round of the top-k
+// is then a maximum over registers and three shuffles; only the lane that holds
+// the best score looks into shared memory, at 8 values, and takes it out.  Equal
+// scores go to the lowest lane and the lowest place in it: the lowest expert.
+// What bounds this is the issue of instructions, not memory: rounds by a whole
+// warp a token, rescanning its scores each time, took 172 us for 65,536 tokens
+// x 256 experts (sigmoid, bias, 4 of 8 groups, k = 8) against ROUTE_US here.
+//
+// -inf stands for an expert that cannot be chosen.  NaN takes no part in the
+// rounds (fmaxf passes over it): a row that has one picks its NaN first, in a
+// loop that other rows do not enter.
+//
+// Backward.  The row of gradients is built in shared memory from the k chosen
+// experts, the softmax's two sums run over registers.
 #include "rows.cuh"
 
 namespace bgl {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxChoices = 32, kMaxGroups = 32;
-constexpr int kWarps = 4;  // tokens of a block
+constexpr int kLanes = 8;            // lanes of a token
+constexpr int kTokens = 32 / kLanes; // tokens of a warp
+constexpr int kWarps = 4;            // warps of a block
+// of a block that selects among `subs` * 64 experts: fewer where shared memory would not do
+__host__ __device__ constexpr int select_warps(int subs) { return subs > 8 ? 2 : kWarps; }
 
 struct RouteArgs {
     const void *logits;
@@ -30,14 +46,37 @@ __device__ __forceinline__ uint32_t key_of(float c) {
     const uint32_t u = __float_as_uint(__fadd_rn(c, 0.0f));
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);
+
+// Maximum and sum over the LANES lanes of a token, on each of them.
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+// Four logits at once.
+__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+    const float4 x = __ldg(reinterpret_cast<const float4 *>(p));
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float (&v)[4]) {
+    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+    v[0] = __uint_as_float(x.x << 16), v[1] = __uint_as_float(x.x & 0xffff0000u);
+    v[2] = __uint_as_float(x.y << 16), v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float *p, const float (&v)[4]) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&v)[4]) {
+    __nv_bfloat162 o[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(o);
 }
 
 // A sum of weights to divide by: the smallest normal number where all of them
@@ -47,96 +86,191 @@ __device__ __forceinline__ float at_least_tiny(float sum) {
 }
 
 // 1 / (1 + exp(-x)), every step rounded once.
-__device__ __forceinline__ float sigmoid_of(float x) {
-    return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-x)));
-}
+__device__ __forceinline__ float sigmoid_of(float x) { return __frcp_rn(__fadd_rn(1.0f, expf(-x))); }
 
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) k_route_topk(const RouteArgs a) {
-    extern __shared__ uint32_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t *key = smem + warp * a.experts;
-    const int per_group = a.experts / a.groups;
-    for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < a.tokens;
-         t += (int64_t)gridDim.x * kWarps) {
-        const T *x = static_cast<const T *>(a.logits) + t * a.experts;
-        float top = -INFINITY, total = 0;
-        if (!a.sigmoid) {
-            for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, to_acc(x[e]));
-            top = warp_max(top);
+// SUBS * 8 experts a lane; VEC: rows in 16-byte (bf16: 8-byte) pieces.
+template <typename T, int SUBS, bool VEC>
+__global__ void __launch_bounds__(select_warps(SUBS) * 32) k_route_topk(const RouteArgs a) {
+    constexpr int kSlots = select_warps(SUBS) * kTokens;
+    constexpr int kOwn = SUBS * 8;          // experts of a lane
+    constexpr int kStride = kOwn + 4;       // apart in shared memory: no bank conflicts
+    constexpr int kRow = kLanes * kStride;  // a token's scores
+    __shared__ __align__(16) float scores[kSlots][kRow];
+    __shared__ uint32_t groups[kSlots][kMaxGroups];
+    __shared__ int picked[kSlots][kMaxChoices];
+    const int lane = threadIdx.x & 31, own = lane & (kLanes - 1);
+    const int slot = threadIdx.x / kLanes;
+    float *c = scores[slot], *mine = c + own * kStride;
+    int *pick = picked[slot];
+    const int experts = a.experts, per_group = experts / a.groups;
+    auto at = [](int e) { return e + e / kOwn * 4; };  // expert e's place in c
+    const bool need_sum = !a.sigmoid && !(a.by_logit && a.renormalize);
+
+    for (int64_t t0 = (int64_t)blockIdx.x * kSlots; t0 < a.tokens; t0 += (int64_t)gridDim.x * kSlots) {
+        // lanes behind the last token repeat it and write nothing
+        const bool live = t0 + slot < a.tokens;
+        const int64_t t = live ? t0 + slot : a.tokens - 1;
+        const T *x = static_cast<const T *>(a.logits) + t * experts;
+
+        // the token's logits: piece own + 8 i of four (VEC), or one by one
+        constexpr int kPieces = VEC ? kOwn / 4 : kOwn, kWide = VEC ? 4 : 1;
+        float l[kPieces][kWide];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = (own + kLanes * i) * kWide;
+            if (e < experts) {
+                if constexpr (VEC) load4(x + e, l[i]);
+                else l[i][0] = to_acc(x[e]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) l[i][j] = -INFINITY;
+            }
+        }
+        float top = 0, total = 1;
+        if (need_sum) {
+            top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) top = fmaxf(top, l[i][j]);
+            top = lanes_max<kLanes>(top);
             if (top == -INFINITY) top = 0;
-            for (int e = lane; e < a.experts; e += 32) total += expf(to_acc(x[e]) - top);
-            total = warp_sum(total);
+            total = 0;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) total += expf(l[i][j] - top);
+            total = lanes_sum<kLanes>(total);
         }
-        for (int e = lane; e < a.experts; e += 32) {
-            const float l = to_acc(x[e]);
-            float c = l;
-            if (!a.by_logit) {
-                c = a.sigmoid ? sigmoid_of(l) : expf(l - top) / total;
-                if (a.bias) c = __fadd_rn(c, a.bias[e]);
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = (own + kLanes * i) * kWide;
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) {
+                float v = l[i][j];
+                if (!a.by_logit && e < experts) {
+                    float s = a.sigmoid ? sigmoid_of(v) : expf(v - top) / total;
+                    if (a.bias) s = __fadd_rn(s, __ldg(a.bias + e + j));
+                    v = v == -INFINITY ? v : s;
+                }
+                nan |= v != v;
+                l[i][j] = v;
             }
-            key[e] = (l == -INFINITY || c == -INFINITY) ? 0u : key_of(c);
+            if constexpr (VEC) store4(c + at(e), l[i]);
+            else c[at(e)] = l[i][0];
         }
+        const unsigned nans = __ballot_sync(0xffffffffu, nan);
         __syncwarp();
+
         if (a.groups > 1) {
-            uint32_t best = 0;
-            if (lane < a.groups) {
-                uint32_t k1 = 0, k2 = 0;
+            for (int g = own; g < a.groups; g += kLanes) {
+                float k1 = -INFINITY, k2 = -INFINITY;
+                bool bad = false;
                 for (int i = 0; i < per_group; ++i) {
-                    const uint32_t k = key[lane * per_group + i];
-                    if (k > k1) {
-                        k2 = k1;
-                        k1 = k;
-                    } else if (k > k2) {
-                        k2 = k;
-                    }
+                    const float v = c[at(g * per_group + i)];
+                    bad |= v != v;
+                    k2 = fmaxf(k2, fminf(k1, v));
+                    k1 = fmaxf(k1, v);
                 }
-                best = k1;
-                if (a.group_top == 2 && k2) best = key_of(__fadd_rn(value_of(k1), value_of(k2)));
+                // 0: nothing to choose in this group
+                uint32_t key = k1 == -INFINITY ? 0u : key_of(k1);
+                if (a.group_top == 2 && k2 > -INFINITY) key = key_of(__fadd_rn(k1, k2));
+                groups[slot][g] = bad ? 0xffffffffu : key;
             }
-            int rank = 0;
-            for (int g = 0; g < a.groups; ++g) {
-                const uint32_t other = __shfl_sync(0xffffffffu, best, g);
-                rank += other > best || (other == best && g < lane);
+            __syncwarp();
+            for (int g = own; g < a.groups; g += kLanes) {
+                const uint32_t key = groups[slot][g];
+                int rank = 0;
+                for (int o = 0; o < a.groups; ++o) {
+                    const uint32_t other = groups[slot][o];
+                    rank += other > key || (other == key && o < g);
+                }
+                if (rank >= a.topk_groups)
+                    for (int i = 0; i < per_group; ++i) c[at(g * per_group + i)] = -INFINITY;
             }
-            if (lane < a.groups && rank >= a.topk_groups)
-                for (int i = 0; i < per_group; ++i) key[lane * per_group + i] = 0;
             __syncwarp();
         }
-        int mine = -1;
+
+        // the maxima of the lane's own experts, 8 by 8
+        float sub[SUBS];
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+            const float4 u = *reinterpret_cast<float4 *>(mine + 8 * s);
+            const float4 v = *reinterpret_cast<float4 *>(mine + 8 * s + 4);
+            sub[s] = fmaxf(fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)), fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        }
+        int first = 0;  // places taken by NaN
+        if (nans) {
+            if (own == 0 && (nans >> (lane & 24) & 0xffu))
+                for (int e = 0; e < experts && first < a.k; ++e)
+                    if (c[at(e)] != c[at(e)]) pick[first++] = e;
+            first = __shfl_sync(0xffffffffu, first, lane & 24);
+        }
         for (int j = 0; j < a.k; ++j) {
-            uint32_t best = 0;
-            int at = a.experts;
-            for (int e = lane; e < a.experts; e += 32)
-                if (key[e] > best) {
-                    best = key[e];
-                    at = e;
-                }
-            const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
-            if (top_key == 0) break;
-            const int e = __reduce_min_sync(0xffffffffu, best == top_key ? at : a.experts);
-            if (lane == j) mine = e;
-            if (lane == (e & 31)) key[e] = 0;
-            __syncwarp();
+            float best = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) best = fmaxf(best, sub[s]);
+            const float m = lanes_max<kLanes>(best);
+            const unsigned holders = __ballot_sync(0xffffffffu, best == m) >> (lane & 24) & 0xffu;
+            if (j < first) continue;
+            if (m == -INFINITY) {
+                if (own == 0) pick[j] = -1;
+            } else if (own == __ffs(holders) - 1) {
+                int s = 0;
+#pragma unroll
+                for (int i = SUBS - 1; i >= 0; --i)
+                    if (sub[i] == m) s = i;
+                float v[8];
+                const float4 lo = *reinterpret_cast<float4 *>(mine + 8 * s);
+                const float4 hi = *reinterpret_cast<float4 *>(mine + 8 * s + 4);
+                v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+                v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+                int place = 0;
+#pragma unroll
+                for (int i = 7; i >= 0; --i)
+                    if (v[i] == m) place = i;
+                float rest = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rest = fmaxf(rest, i == place ? -INFINITY : v[i]);
+                mine[8 * s + place] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < SUBS; ++i)
+                    if (i == s) sub[i] = rest;
+                pick[j] = own * kOwn + 8 * s + place;
+            }
         }
         __syncwarp();
-        const float l = mine >= 0 ? to_acc(x[mine]) : -INFINITY;
-        float w = 0;
-        if (a.sigmoid) {
-            w = mine >= 0 ? sigmoid_of(l) : 0.0f;
-            if (a.renormalize) w = w / at_least_tiny(warp_sum(w));
-        } else if (a.renormalize) {
-            const float m = warp_max(l);
-            w = mine >= 0 ? expf(l - m) : 0.0f;
-            const float sum = warp_sum(w);
-            if (mine >= 0) w /= sum;
-        } else if (mine >= 0) {
-            w = expf(l - top) / total;
+
+        // weights: lane i has the choices i, i + 8, ...
+        constexpr int kEach = kMaxChoices / kLanes;
+        float w[kEach];
+        float sum = 0, most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int j = own + kLanes * i, e = j < a.k ? pick[j] : -1;
+            w[i] = e >= 0 ? to_acc(x[e]) : -INFINITY;
+            most = fmaxf(most, w[i]);
         }
-        if (lane < a.k) {
-            a.weights[t * a.k + lane] = mine >= 0 ? w * a.scale : 0.0f;
-            a.indices[t * a.k + lane] = mine;
+        if (!a.sigmoid) most = a.renormalize ? lanes_max<kLanes>(most) : top;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int j = own + kLanes * i;
+            const bool chosen = j < a.k && pick[j] >= 0;
+            w[i] = !chosen ? 0.0f : a.sigmoid ? sigmoid_of(w[i]) : expf(w[i] - most);
+            sum += w[i];
         }
+        if (a.renormalize) total = at_least_tiny(lanes_sum<kLanes>(sum));
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int j = own + kLanes * i;
+            if (j >= a.k || !live) continue;
+            const int e = pick[j];
+            if (e >= 0 && (a.renormalize || !a.sigmoid)) w[i] /= total;
+            a.weights[t * a.k + j] = e >= 0 ? w[i] * a.scale : 0.0f;
+            a.indices[t * a.k + j] = e;
+        }
+        __syncwarp();
     }
 }
 
@@ -151,62 +285,173 @@ struct RouteGradArgs {
     void *dlogits;
 };
 
-template <typename T>
+// LANES lanes a token, PER experts a lane, in pieces of four (VEC) or one.
+template <typename T, int LANES, int PER, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) k_route_topk_backward(const RouteGradArgs a) {
-    extern __shared__ float sums[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float *acc = sums + warp * a.experts;
-    for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < a.tokens;
-         t += (int64_t)gridDim.x * kWarps) {
-        const T *x = static_cast<const T *>(a.logits) + t * a.experts;
-        T *dx = static_cast<T *>(a.dlogits) + t * a.experts;
-        int64_t at = lane < a.k ? a.indices[t * a.k + lane] : -1;
-        if (at >= a.experts) at = -1;
-        const bool chosen = at >= 0;
-        float g = chosen ? a.grad[t * a.k + lane] * a.scale : 0.0f;
-        const float l = chosen ? to_acc(x[at]) : -INFINITY;
-        const bool dense = !a.sigmoid && !a.renormalize;
-        if (a.sigmoid) {
-            const float s = chosen ? sigmoid_of(l) : 0.0f;
+    constexpr int kSlots = kWarps * 32 / LANES;
+    constexpr int kWide = VEC ? 4 : 1, kPieces = PER / kWide;
+    constexpr int kEach = kMaxChoices / LANES > 0 ? kMaxChoices / LANES : 1;  // choices of a lane
+    __shared__ __align__(16) float sums[kSlots][LANES * PER];
+    const int lane = threadIdx.x & 31, own = lane & (LANES - 1), slot = threadIdx.x / LANES;
+    const int experts = a.experts;
+    const bool dense = !a.sigmoid && !a.renormalize;
+    float *acc = sums[slot];
+    for (int64_t t0 = (int64_t)blockIdx.x * kSlots; t0 < a.tokens; t0 += (int64_t)gridDim.x * kSlots) {
+        // lanes behind the last token repeat it and write nothing
+        const bool live = t0 + slot < a.tokens;
+        const int64_t t = live ? t0 + slot : a.tokens - 1;
+        const T *x = static_cast<const T *>(a.logits) + t * experts;
+        T *dx = static_cast<T *>(a.dlogits) + t * experts;
+        float l[kPieces][kWide];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = (own + LANES * i) * kWide;
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) l[i][j] = -INFINITY;
+            if (dense && e < experts) {
+                if constexpr (VEC) load4(x + e, l[i]);
+                else l[i][0] = to_acc(x[e]);
+            }
+        }
+        int at[kEach];
+        float g[kEach], s[kEach];
+        float most = -INFINITY, total = 0, dot = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int j = own + LANES * i;
+            const int64_t e = j < a.k ? a.indices[t * a.k + j] : -1;
+            at[i] = e >= 0 && e < experts ? (int)e : -1;
+            g[i] = at[i] >= 0 ? a.grad[t * a.k + j] * a.scale : 0.0f;
+            s[i] = at[i] >= 0 && !dense ? to_acc(x[at[i]]) : -INFINITY;
+            most = fmaxf(most, s[i]);
+        }
+        if (!dense) {
+            if (!a.sigmoid) most = lanes_max<LANES>(most);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const float logit = s[i];
+                s[i] = at[i] < 0 ? 0.0f : a.sigmoid ? sigmoid_of(logit) : expf(logit - most);
+                total += s[i];
+                dot += at[i] < 0 ? 0.0f : s[i] * g[i];
+                if (a.sigmoid && at[i] >= 0 && !a.renormalize) g[i] *= s[i] * sigmoid_of(-logit);
+                // the slope's other factor, needed again below
+                if (a.sigmoid && at[i] >= 0 && a.renormalize) s[i] *= sigmoid_of(-logit);
+            }
             if (a.renormalize) {
-                const float total = at_least_tiny(warp_sum(s));
-                g = (g - warp_sum(g * s) / total) / total;
+                total = at_least_tiny(lanes_sum<LANES>(total));
+                dot = lanes_sum<LANES>(dot) / total;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    if (at[i] >= 0) g[i] = s[i] / total * (g[i] - dot);
             }
-            g = chosen ? g * (s * sigmoid_of(-l)) : 0.0f;
-        } else if (a.renormalize) {
-            const float m = warp_max(l);
-            const float p = chosen ? expf(l - m) : 0.0f;
-            const float w = p / warp_sum(p);
-            const float mean = warp_sum(chosen ? w * g : 0.0f);
-            g = chosen ? w * (g - mean) : 0.0f;
         }
-        for (int e = lane; e < a.experts; e += 32) acc[e] = 0;
+        // the row of the chosen experts' values, zero elsewhere
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i)
+            *reinterpret_cast<float4 *>(acc + (own + LANES * i) * 4) = make_float4(0, 0, 0, 0);
         __syncwarp();
-        // one choice after the other: indices given twice add up in order
-        for (int j = 0; j < a.k; ++j) {
-            if (lane == j && chosen) acc[at] += g;
+        // an expert that is given twice shows where the numbers of its places meet
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (at[i] >= 0) acc[at[i]] = __int_as_float(own + LANES * i);
+        __syncwarp();
+        bool twice = false;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            twice |= at[i] >= 0 && __float_as_int(acc[at[i]]) != own + LANES * i;
+        twice = __any_sync(0xffffffffu, twice);
+        if (!twice) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (at[i] >= 0) acc[at[i]] = g[i];
+        } else {  // one place after the other: they add up in order
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (at[i] >= 0) acc[at[i]] = 0;
             __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                for (int o = 0; o < LANES; ++o) {
+                    if (own == o && at[i] >= 0) acc[at[i]] += g[i];
+                    __syncwarp();
+                }
         }
+        __syncwarp();
         if (dense) {
-            float top = -INFINITY, total = 0, dot = 0;
-            for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, to_acc(x[e]));
-            top = warp_max(top);
-            if (top == -INFINITY) top = 0;
-            for (int e = lane; e < a.experts; e += 32) {
-                const float p = expf(to_acc(x[e]) - top);
-                total += p;
-                dot += p * acc[e];
-            }
-            total = warp_sum(total);
+            most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) most = fmaxf(most, l[i][j]);
+            most = lanes_max<LANES>(most);
+            if (most == -INFINITY) most = 0;
+            total = dot = 0;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    l[i][j] = expf(l[i][j] - most);
+                    total += l[i][j];
+                    dot += l[i][j] * acc[(own + LANES * i) * kWide + j];
+                }
+            total = lanes_sum<LANES>(total);
             if (total == 0) total = 1;  // every expert masked: no gradient
-            dot = warp_sum(dot) / total;
-            for (int e = lane; e < a.experts; e += 32)
-                dx[e] = from_acc<T>(expf(to_acc(x[e]) - top) / total * (acc[e] - dot));
-        } else {
-            for (int e = lane; e < a.experts; e += 32) dx[e] = from_acc<T>(acc[e]);
+            dot = lanes_sum<LANES>(dot) / total;
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = (own + LANES * i) * kWide;
+            float v[kWide];
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) {
+                v[j] = acc[e + j];
+                if (dense) v[j] = l[i][j] / total * (v[j] - dot);
+            }
+            if (e < experts && live) {
+                if constexpr (VEC) store4(dx + e, v);
+                else dx[e] = from_acc<T>(v[0]);
+            }
         }
         __syncwarp();
     }
+}
+
+template <typename T, int SUBS>
+void launch_topk(const RouteArgs &a, cudaStream_t s) {
+    constexpr int threads = select_warps(SUBS) * 32;
+    const bool vec = a.experts % 4 == 0 && aligned(a.logits, 4 * sizeof(T));
+    const int64_t want = (a.tokens * kLanes + threads - 1) / threads;
+    const unsigned blocks = (unsigned)(want < (1 << 20) ? want : 1 << 20);
+    if (vec) k_route_topk<T, SUBS, true><<<blocks, threads, 0, s>>>(a);
+    else k_route_topk<T, SUBS, false><<<blocks, threads, 0, s>>>(a);
+}
+// The fewest 64s of experts that hold the row (a lane's registers grow with them).
+template <typename T>
+void launch_topk(const RouteArgs &a, cudaStream_t s) {
+    if (a.experts <= 64) launch_topk<T, 1>(a, s);
+    else if (a.experts <= 128) launch_topk<T, 2>(a, s);
+    else if (a.experts <= 256) launch_topk<T, 4>(a, s);
+    else if (a.experts <= 512) launch_topk<T, 8>(a, s);
+    else launch_topk<T, 16>(a, s);
+}
+
+template <typename T, int LANES, int PER>
+void launch_backward(const RouteGradArgs &a, cudaStream_t s) {
+    const bool vec = a.experts % 4 == 0 && aligned(a.logits, 4 * sizeof(T)) && aligned(a.dlogits, 4 * sizeof(T));
+    constexpr int64_t slots = kWarps * 32 / LANES;
+    const int64_t want = (a.tokens + slots - 1) / slots;
+    const unsigned blocks = (unsigned)(want < (1 << 20) ? want : 1 << 20);
+    if (vec) k_route_topk_backward<T, LANES, PER, true><<<blocks, kWarps * 32, 0, s>>>(a);
+    else k_route_topk_backward<T, LANES, PER, false><<<blocks, kWarps * 32, 0, s>>>(a);
+}
+// Eight experts a lane while that leaves whole tokens to a warp.
+template <typename T>
+void launch_backward(const RouteGradArgs &a, cudaStream_t s) {
+    if (a.experts <= 64) launch_backward<T, 8, 8>(a, s);
+    else if (a.experts <= 128) launch_backward<T, 16, 8>(a, s);
+    else if (a.experts <= 256) launch_backward<T, 32, 8>(a, s);
+    else if (a.experts <= 512) launch_backward<T, 32, 16>(a, s);
+    else launch_backward<T, 32, 32>(a, s);
 }
 
 int check_route(const char *who, int64_t tokens, int64_t experts, int64_t k, int score, int dtype) {
@@ -219,11 +464,6 @@ int check_route(const char *who, int64_t tokens, int64_t experts, int64_t k, int
     if (k < 1 || k > experts) return fail(BGL_E_INVALID, "%s: k must be in [1, experts]", who);
     if (k > kMaxChoices) return fail(BGL_E_UNSUPPORTED, "%s: k above %d", who, kMaxChoices);
     return BGL_OK;
-}
-
-unsigned blocks_for(int64_t tokens) {
-    const int64_t want = (tokens + kWarps - 1) / kWarps, cap = (int64_t)num_sms() * 16;
-    return (unsigned)(want < cap ? want : cap);
 }
 
 }  // namespace
@@ -267,11 +507,8 @@ int bgl_route_topk(const void *logits, const float *bias, int64_t tokens, int64_
     a.scale = (float)scale;
     a.weights = weights;
     a.indices = indices;
-    const size_t smem = (size_t)kWarps * experts * sizeof(uint32_t);
-    if (dtype == BGL_F32)
-        k_route_topk<float><<<blocks_for(tokens), kWarps * 32, smem, as_stream(stream)>>>(a);
-    else
-        k_route_topk<__nv_bfloat16><<<blocks_for(tokens), kWarps * 32, smem, as_stream(stream)>>>(a);
+    if (dtype == BGL_F32) launch_topk<float>(a, as_stream(stream));
+    else launch_topk<__nv_bfloat16>(a, as_stream(stream));
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }
@@ -295,12 +532,8 @@ int bgl_route_topk_backward(const float *grad, const void *logits, const int64_t
     a.renormalize = renormalize != 0;
     a.scale = (float)scale;
     a.dlogits = dlogits;
-    const size_t smem = (size_t)kWarps * experts * sizeof(float);
-    if (dtype == BGL_F32)
-        k_route_topk_backward<float><<<blocks_for(tokens), kWarps * 32, smem, as_stream(stream)>>>(a);
-    else
-        k_route_topk_backward<__nv_bfloat16>
-            <<<blocks_for(tokens), kWarps * 32, smem, as_stream(stream)>>>(a);
+    if (dtype == BGL_F32) launch_backward<float>(a, as_stream(stream));
+    else launch_backward<__nv_bfloat16>(a, as_stream(stream));
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }
