@@ -95,6 +95,22 @@ __device__ __forceinline__ A group_sum(A v, A (*smem)[kThreads / 32 + 1], int &t
     return v;
 }
 
+// Both sums at once, with one barrier.
+template <int GROUP, typename A>
+__device__ __forceinline__ void group_sums(A &u, A &v, A (*smem)[2 * (kThreads / 32)], int &turn) {
+    u = warp_sum(u);
+    v = warp_sum(v);
+    if constexpr (GROUP > 32) {
+        const int warp = threadIdx.x >> 5, first = warp / (GROUP / 32) * (GROUP / 32);
+        if ((threadIdx.x & 31) == 0) smem[turn][2 * warp] = u, smem[turn][2 * warp + 1] = v;
+        __syncthreads();
+        u = v = 0;
+#pragma unroll
+        for (int i = 0; i < GROUP / 32; ++i) u += smem[turn][2 * (first + i)], v += smem[turn][2 * (first + i) + 1];
+        turn ^= 1;
+    }
+}
+
 template <typename T, typename W, int GROUP, int N, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     k_layer_norm(const T *__restrict__ x, const W *__restrict__ w, const W *__restrict__ b,
@@ -169,7 +185,26 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows
+// Rows of x and dy that are under way for each group: stages of a ring in
+// shared memory, as many as two blocks an SM (one, of rows of 32 values a thread)
+// have room for.  A thread copies and reads its own pieces only, so its
+// cp.async groups are all the synchronisation there is.
+template <typename T, int N>
+__host__ __device__ constexpr int ring_stages() {
+    constexpr int bytes = kThreads * 2 * N * (int)sizeof(T);
+    constexpr int n = (N * (int)sizeof(T) > 64 ? 196608 : 98304) / bytes;
+    return n > 4 ? 4 : n;
+}
+template <typename T, int GROUP, int N, bool VEC>
+constexpr size_t backward_smem() {
+    // the ring, or the columns where the block's groups meet at the end
+    const size_t ring = VEC ? (size_t)ring_stages<T, N>() * kThreads * 2 * N * sizeof(T) : 0;
+    const size_t columns = GROUP < kThreads ? (size_t)GROUP * N * sizeof(Acc<T>) : 0;
+    return ring > columns ? ring : columns;
+}
+
+// partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows,
+// which are consecutive
 template <typename T, typename W, int GROUP, int N, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     k_layer_norm_backward(const T *__restrict__ dy, const T *__restrict__ x,
@@ -178,13 +213,14 @@ __global__ void __launch_bounds__(kThreads)
                           Acc<T> *__restrict__ partial) {
     using A = Acc<T>;
     using H = Held<T, N, VEC>;
-    constexpr int kGroups = kThreads / GROUP;
-    __shared__ A smem[2][kThreads / 32 + 1];
-    extern __shared__ __align__(16) unsigned char raw_columns[];
-    A *columns = reinterpret_cast<A *>(raw_columns);  // [GROUP * N] where a block has several groups
+    constexpr int kGroups = kThreads / GROUP, kStages = ring_stages<T, N>();
+    __shared__ A smem[2][2 * (kThreads / 32)];
+    extern __shared__ __align__(16) unsigned char raw[];
+    A *columns = reinterpret_cast<A *>(raw);  // [GROUP * N], after the rows
+    uint4 *ring = reinterpret_cast<uint4 *>(raw);  // [stage][x, dy][piece][thread]
     int turn = 0;
     const int t = threadIdx.x % GROUP;
-    const int64_t stride = (int64_t)gridDim.x * kGroups, first = (int64_t)blockIdx.x * kGroups;
+    const int64_t begin = rows * blockIdx.x / gridDim.x, end = rows * (blockIdx.x + 1) / gridDim.x;
     A aw[H::kPieces][H::kWide], ab[H::kPieces][H::kWide], wv[H::kPieces][H::kWide];
 #pragma unroll
     for (int i = 0; i < H::kPieces; ++i) {
@@ -193,24 +229,49 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < H::kWide; ++j) aw[i][j] = ab[i][j] = 0, wv[i][j] = 1;
         if (w && e < d) load_params<W, H::kWide, VEC>(w + e, wv[i]);
     }
-    H next_x, next_g;
-    A next_mu = 0, next_rs = 0;
-    int64_t row = first + threadIdx.x / GROUP;
-    auto fetch = [&](int64_t r) {
-        if (r >= rows) return;
-        next_x.template load<GROUP>(x + r * d, t, d);
-        next_g.template load<GROUP>(dy + r * d, t, d);
-        next_mu = mean[r], next_rs = rstd[r];
+    int64_t row = begin + threadIdx.x / GROUP;
+    auto fetch = [&](int64_t r, int stage) {
+        if constexpr (VEC) {
+            if (r < end)
+#pragma unroll
+                for (int i = 0; i < H::kPieces; ++i) {
+                    const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
+                    if (e >= d) continue;
+                    uint4 *slot = ring + ((stage * 2) * H::kPieces + i) * kThreads + threadIdx.x;
+                    cp_async<16>(smem_addr(slot), x + r * d + e);
+                    cp_async<16>(smem_addr(slot + H::kPieces * kThreads), dy + r * d + e);
+                }
+            cp_async_commit();  // an empty group where there is no row: the count stays
+        }
     };
-    fetch(row);
-    for (int64_t r0 = first; r0 < rows; r0 += stride, row += stride) {
-        const H hx = next_x, hg = next_g;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(row + i * kGroups, i);
+    int stage = 0;
+    A next_mu = row < end ? mean[row] : A(0), next_rs = row < end ? rstd[row] : A(0);
+    for (int64_t r0 = begin; r0 < end; r0 += kGroups, row += kGroups) {
+        const bool live = row < end;
+        H hx, hg;
+        if constexpr (VEC) {
+            // into the stage that was read last time
+            fetch(row + (kStages - 1) * kGroups, stage == 0 ? kStages - 1 : stage - 1);
+            cp_async_wait<kStages - 1>();
+#pragma unroll
+            for (int i = 0; i < H::kPieces; ++i) {
+                const uint4 *slot = ring + ((stage * 2) * H::kPieces + i) * kThreads + threadIdx.x;
+                hx.p[i].raw = slot[0];
+                hg.p[i].raw = slot[H::kPieces * kThreads];
+            }
+            stage = stage == kStages - 1 ? 0 : stage + 1;
+        } else if (live) {
+            hx.template load<GROUP>(x + row * d, t, d);
+            hg.template load<GROUP>(dy + row * d, t, d);
+        }
         const A mu = next_mu, rs = next_rs;
-        fetch(row + stride);
+        if (row + kGroups < end) next_mu = mean[row + kGroups], next_rs = rstd[row + kGroups];
         A s1 = 0, s2 = 0;
 #pragma unroll
         for (int i = 0; i < H::kPieces; ++i) {
-            if ((int64_t)(t + GROUP * i) * H::kWide >= d || row >= rows) continue;
+            if ((int64_t)(t + GROUP * i) * H::kWide >= d || !live) continue;
 #pragma unroll
             for (int j = 0; j < H::kWide; ++j) {
                 const A g = hg.at(i, j), xhat = (hx.at(i, j) - mu) * rs, v = g * wv[i][j];
@@ -220,9 +281,10 @@ __global__ void __launch_bounds__(kThreads)
                 s2 += v * xhat;
             }
         }
-        s1 = group_sum<GROUP>(s1, smem, turn) / A(d);
-        s2 = group_sum<GROUP>(s2, smem, turn) / A(d);
-        if (row >= rows || !dx) continue;
+        group_sums<GROUP>(s1, s2, smem, turn);
+        s1 /= A(d);
+        s2 /= A(d);
+        if (!live || !dx) continue;
 #pragma unroll
         for (int i = 0; i < H::kPieces; ++i) {
             const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
@@ -237,6 +299,7 @@ __global__ void __launch_bounds__(kThreads)
             else dx[row * d + e] = o.v[0];
         }
     }
+    if constexpr (VEC) cp_async_wait<0>();
     if (!partial) return;
     // the block's groups one after the other, then the block's row of partials
 #pragma unroll
@@ -358,13 +421,13 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Adds the partial rows: 32 columns a block, the parts eight ways, both in a
-// fixed order.  blockIdx.y: 0 dw, 1 db.
+// Adds the partial rows: 32 columns a block, the parts 32 ways, both in a fixed
+// order.  blockIdx.y: 0 dw, 1 db.
 template <typename A, typename W>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(1024)
     k_layer_norm_join(const A *__restrict__ partial, int64_t parts, int64_t d, W *__restrict__ dw,
                       W *__restrict__ db) {
-    __shared__ A sums[8][33];
+    __shared__ A sums[32][33];
     W *out = blockIdx.y ? db : dw;
     if (!out) return;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -373,14 +436,13 @@ __global__ void __launch_bounds__(kThreads)
     if (col < d) {
         const A *p = partial + blockIdx.y * d + col;
 #pragma unroll 8
-        for (int64_t i = ty; i < parts; i += 8) s += p[i * 2 * d];
+        for (int64_t i = ty; i < parts; i += 32) s += p[i * 2 * d];
     }
     sums[ty][tx] = s;
     __syncthreads();
-    if (ty == 0 && col < d) {
-        for (int i = 1; i < 8; ++i) s += sums[i][tx];
-        out[col] = from_acc<W>(Acc<W>(s));
-    }
+    s = warp_sum(sums[tx][ty]);  // warp ty adds column ty
+    const int64_t mine = (int64_t)blockIdx.x * 32 + ty;
+    if (tx == 0 && mine < d) out[mine] = from_acc<W>(Acc<W>(s));
 }
 
 int64_t split_rows_of(int64_t rows) {
@@ -512,19 +574,23 @@ int backward(const Backward &p) {
         const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) && aligned(w, 16);
         const int rc = with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
             constexpr int G = decltype(c)::group, N = decltype(c)::values;
-            const size_t smem = G < kThreads ? (size_t)G * N * sizeof(A) : 0;
             const unsigned grid = (unsigned)parts;
-            if (vec)
+            constexpr size_t smem = backward_smem<T, G, N, true>(), plain = backward_smem<T, G, N, false>();
+            if (vec) {
+                if (smem > 48 * 1024)
+                    BGL_CUDA(cudaFuncSetAttribute(k_layer_norm_backward<T, W, G, N, true>,
+                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
                 k_layer_norm_backward<T, W, G, N, true><<<grid, kThreads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
-            else
-                k_layer_norm_backward<T, W, G, N, false><<<grid, kThreads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
+            } else {
+                k_layer_norm_backward<T, W, G, N, false><<<grid, kThreads, plain, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
+            }
             BGL_LAUNCH_CHECK();
             return (int)BGL_OK;
         });
         if (rc) return rc;
     }
     if (sums) {
-        k_layer_norm_join<A, W><<<dim3((unsigned)((p.d + 31) / 32), 2), kThreads, 0, p.s>>>(
+        k_layer_norm_join<A, W><<<dim3((unsigned)((p.d + 31) / 32), 2), 1024, 0, p.s>>>(
             partial, parts, p.d, (W *)p.dw, (W *)p.db);
         BGL_LAUNCH_CHECK();
     }
