@@ -23,160 +23,210 @@ namespace bgl {
 namespace {
 
 constexpr int kThreads = 256;
+// A block has 256 threads, or one group where that is larger.
+__host__ __device__ constexpr int threads_of(int group) { return group > kThreads ? group : kThreads; }
 constexpr int kMostHeld = 8192;    // values of a row that registers hold
 constexpr int kSplitRows = 256;    // longer rows: rows of one partial sum, at least
 constexpr int kMaxSplits = 256;
 
-// `N` values at p, 16 bytes at a time where VEC; as they are in memory, so that
-// loads in flight take few registers.
-template <typename T, int N, bool VEC>
-struct Held {
-    static constexpr int kWide = VEC ? 16 / (int)sizeof(T) : 1;
-    static constexpr int kPieces = N / kWide;
-    union Piece {
-        uint4 raw;
-        T v[kWide];
-        __device__ Piece() {}
-    };
-    Piece p[kPieces];
-
-    // piece i of thread t of a group: values (t + GROUP i) * kWide and on
-    template <int GROUP>
-    __device__ __forceinline__ void load(const T *row, int t, int64_t d) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int64_t e = (int64_t)(t + GROUP * i) * kWide;
-            if (e < d) {
-                if constexpr (VEC) p[i].raw = __ldcs(reinterpret_cast<const uint4 *>(row + e));
-                else p[i].v[0] = row[e];
-            }
-        }
-    }
-    __device__ __forceinline__ Acc<T> at(int i, int j) const { return to_acc(p[i].v[j]); }
+// Two values that are worked on together.  float32 pairs go through the packed
+// instructions (one issue for two operations, each rounded as alone): the bf16
+// kernels are bound by issue, not by memory, without them.
+template <typename A>
+struct Pair {
+    A x, y;
 };
+__device__ __forceinline__ unsigned long long bits(Pair<float> p) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(p.x), "f"(p.y));
+    return r;
+}
+__device__ __forceinline__ Pair<float> pair(unsigned long long b) {
+    Pair<float> p;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(p.x), "=f"(p.y) : "l"(b));
+    return p;
+}
+__device__ __forceinline__ Pair<float> operator+(Pair<float> a, Pair<float> b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+__device__ __forceinline__ Pair<float> operator*(Pair<float> a, Pair<float> b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+__device__ __forceinline__ Pair<float> fma(Pair<float> a, Pair<float> b, Pair<float> c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair(r);
+}
+__device__ __forceinline__ Pair<double> operator+(Pair<double> a, Pair<double> b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Pair<double> operator*(Pair<double> a, Pair<double> b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Pair<double> fma(Pair<double> a, Pair<double> b, Pair<double> c) {
+    return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
+}
+template <typename A>
+__device__ __forceinline__ Pair<A> both(A v) { return {v, v}; }
 
-// N values of the parameters at p, in 16-byte pieces where VEC.
-template <typename W, int N, bool VEC, typename A>
-__device__ __forceinline__ void load_params(const W *p, A (&v)[N]) {
+// Values of a row as they are in memory: pieces of 16 bytes (VEC), or of one
+// value whose pair partner is zero.
+template <typename T, bool VEC>
+struct Piece {
+    static constexpr int kWide = VEC ? 16 / (int)sizeof(T) : 1;
+    static constexpr int kPairs = VEC ? kWide / 2 : 1;
+    union {
+        uint4 raw;
+        T v[VEC ? kWide : 1];
+    };
+    __device__ Piece() {}
+
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC) raw = __ldcs(reinterpret_cast<const uint4 *>(p));
+        else v[0] = *p;
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (VEC) __stcs(reinterpret_cast<uint4 *>(p), raw);
+        else *p = v[0];
+    }
+    __device__ __forceinline__ Pair<Acc<T>> get(int i) const {
+        if constexpr (VEC) return {to_acc(v[2 * i]), to_acc(v[2 * i + 1])};
+        else return {to_acc(v[0]), Acc<T>(0)};
+    }
+    __device__ __forceinline__ void set(int i, Pair<Acc<T>> p) {
+        if constexpr (VEC) v[2 * i] = from_acc<T>(p.x), v[2 * i + 1] = from_acc<T>(p.y);
+        else v[0] = from_acc<T>(p.x);
+    }
+};
+template <>
+__device__ __forceinline__ void Piece<__nv_bfloat16, true>::set(int i, Pair<float> p) {
+    *reinterpret_cast<__nv_bfloat162 *>(&v[2 * i]) = __floats2bfloat162_rn(p.x, p.y);
+}
+
+// The parameters of a piece at p, in 16-byte loads where VEC.
+template <typename T, bool VEC, typename W>
+__device__ __forceinline__ void load_params(const W *p, Pair<Acc<T>> (&v)[Piece<T, VEC>::kPairs]) {
+    using A = Acc<T>;
     if constexpr (VEC) {
-        constexpr int kWide = 16 / (int)sizeof(W);
-        static_assert(N % kWide == 0, "whole 16-byte pieces");
+        constexpr int kWide = 16 / (int)sizeof(W), kLoads = Piece<T, true>::kWide / kWide;
 #pragma unroll
-        for (int i = 0; i < N / kWide; ++i) {
+        for (int i = 0; i < kLoads; ++i) {
             union {
                 uint4 raw;
                 W w[kWide];
             } u;
             u.raw = __ldg(reinterpret_cast<const uint4 *>(p) + i);
 #pragma unroll
-            for (int j = 0; j < kWide; ++j) v[i * kWide + j] = A(to_acc(u.w[j]));
+            for (int j = 0; j < kWide / 2; ++j)
+                v[i * (kWide / 2) + j] = {A(to_acc(u.w[2 * j])), A(to_acc(u.w[2 * j + 1]))};
         }
     } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = A(to_acc(p[j]));
+        v[0] = {A(to_acc(*p)), A(0)};
     }
 }
 
-// Sum over a group of GROUP threads, on each of them.  Groups of more than a
-// warp are whole blocks' halves, or blocks: `smem` has two values a warp, used in
-// turn so that one barrier a sum is enough.
+// Sums over a group of GROUP threads, on each of them.  A group of more than a
+// warp meets in `smem`, whose two halves are used in turn so that one barrier of
+// the block is enough.
 template <int GROUP, typename A>
-__device__ __forceinline__ A group_sum(A v, A (*smem)[kThreads / 32 + 1], int &turn) {
-    v = warp_sum(v);
-    if constexpr (GROUP > 32) {
-        const int warp = threadIdx.x >> 5, first = warp / (GROUP / 32) * (GROUP / 32);
-        if ((threadIdx.x & 31) == 0) smem[turn][warp] = v;
-        __syncthreads();
-        v = 0;
+__device__ __forceinline__ A lanes_sum(A v) {
 #pragma unroll
-        for (int i = 0; i < GROUP / 32; ++i) v += smem[turn][first + i];
-        turn ^= 1;
-    }
+    for (int o = (GROUP < 32 ? GROUP : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-
-// Both sums at once, with one barrier.
-template <int GROUP, typename A>
-__device__ __forceinline__ void group_sums(A &u, A &v, A (*smem)[2 * (kThreads / 32)], int &turn) {
-    u = warp_sum(u);
-    v = warp_sum(v);
+template <int GROUP, int K, typename A>
+__device__ __forceinline__ void group_sums(A (&v)[K], A (*smem)[K * (threads_of(GROUP) / 32)], int &turn) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lanes_sum<GROUP>(v[k]);
     if constexpr (GROUP > 32) {
         const int warp = threadIdx.x >> 5, first = warp / (GROUP / 32) * (GROUP / 32);
-        if ((threadIdx.x & 31) == 0) smem[turn][2 * warp] = u, smem[turn][2 * warp + 1] = v;
-        __syncthreads();
-        u = v = 0;
 #pragma unroll
-        for (int i = 0; i < GROUP / 32; ++i) u += smem[turn][2 * (first + i)], v += smem[turn][2 * (first + i) + 1];
+        for (int k = 0; k < K; ++k)
+            if ((threadIdx.x & 31) == 0) smem[turn][K * warp + k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = 0;
+#pragma unroll
+        for (int i = 0; i < GROUP / 32; ++i)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += smem[turn][K * (first + i) + k];
         turn ^= 1;
     }
 }
 
 template <typename T, typename W, int GROUP, int N, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(threads_of(GROUP))
     k_layer_norm(const T *__restrict__ x, const W *__restrict__ w, const W *__restrict__ b,
                  int64_t rows, int64_t d, Acc<T> eps, T *__restrict__ y, Acc<T> *__restrict__ mean,
                  Acc<T> *__restrict__ rstd) {
     using A = Acc<T>;
-    using H = Held<T, N, VEC>;
-    constexpr int kGroups = kThreads / GROUP;
-    __shared__ A smem[2][kThreads / 32 + 1];
+    using P = Piece<T, VEC>;
+    constexpr int kGroups = threads_of(GROUP) / GROUP, kPieces = N / P::kWide;
+    __shared__ A smem[2][threads_of(GROUP) / 32];
     int turn = 0;
     const int t = threadIdx.x % GROUP;
-    const int64_t stride = (int64_t)gridDim.x * kGroups;
-    // whole groups take part in the block's barriers even behind the last row
-    const int64_t first = (int64_t)blockIdx.x * kGroups;
-    H next;
+    auto column = [&](int i) { return (t + GROUP * i) * P::kWide; };
+    const int64_t stride = (int64_t)gridDim.x * kGroups, first = (int64_t)blockIdx.x * kGroups;
+    P next[kPieces];
     int64_t row = first + threadIdx.x / GROUP;
-    if (row < rows) next.template load<GROUP>(x + row * d, t, d);
+    auto fetch = [&](int64_t r) {
+        if (r < rows)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                if (column(i) < d) next[i].load(x + r * d + column(i));
+    };
+    fetch(row);
+    // whole groups take part in the block's barriers even behind the last row
     for (int64_t r0 = first; r0 < rows; r0 += stride, row += stride) {
-        const H h = next;
-        if (row + stride < rows) next.template load<GROUP>(x + (row + stride) * d, t, d);
-        A v[H::kPieces][H::kWide];
-        A s = 0;
+        Pair<A> v[kPieces][P::kPairs];
+        Pair<A> s = both(A(0));
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            const bool in = (int64_t)(t + GROUP * i) * H::kWide < d && row < rows;
+        for (int i = 0; i < kPieces; ++i) {
+            const bool in = column(i) < d && row < rows;
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) {
-                v[i][j] = in ? h.at(i, j) : A(0);
-                s += v[i][j];
+            for (int j = 0; j < P::kPairs; ++j) {
+                v[i][j] = in ? next[i].get(j) : both(A(0));
+                s = s + v[i][j];
             }
         }
-        const A mu = group_sum<GROUP>(s, smem, turn) / A(d);
-        s = 0;
+        fetch(row + stride);
+        A sum[1] = {s.x + s.y};
+        group_sums<GROUP>(sum, smem, turn);
+        const A mu = sum[0] / A(d);
+        s = both(A(0));
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            const bool in = (int64_t)(t + GROUP * i) * H::kWide < d;
+        for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) {
-                v[i][j] -= mu;
-                if (in) s += v[i][j] * v[i][j];
+            for (int j = 0; j < P::kPairs; ++j) {
+                v[i][j] = v[i][j] + both(-mu);
+                if (column(i) < d) s = VEC ? fma(v[i][j], v[i][j], s) : Pair<A>{s.x + v[i][j].x * v[i][j].x, 0};
             }
         }
-        const A rs = A(1) / sqrt(group_sum<GROUP>(s, smem, turn) / A(d) + eps);
+        sum[0] = s.x + s.y;
+        group_sums<GROUP>(sum, smem, turn);
+        const A rs = A(1) / sqrt(sum[0] / A(d) + eps);
         if (row >= rows) continue;
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = column(i);
             if (e >= d) continue;
-            A p[H::kWide];
+            Pair<A> p[P::kPairs];
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) v[i][j] *= rs;
+            for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * both(rs);
             if (w) {
-                load_params<W, H::kWide, VEC>(w + e, p);
+                load_params<T, VEC>(w + e, p);
 #pragma unroll
-                for (int j = 0; j < H::kWide; ++j) v[i][j] *= p[j];
+                for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * p[j];
             }
             if (b) {
-                load_params<W, H::kWide, VEC>(b + e, p);
+                load_params<T, VEC>(b + e, p);
 #pragma unroll
-                for (int j = 0; j < H::kWide; ++j) v[i][j] += p[j];
+                for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] + p[j];
             }
-            typename H::Piece o;
+            P o;
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) o.v[j] = from_acc<T>(v[i][j]);
-            if constexpr (VEC) __stcs(reinterpret_cast<uint4 *>(y + row * d + e), o.raw);
-            else y[row * d + e] = o.v[0];
+            for (int j = 0; j < P::kPairs; ++j) o.set(j, v[i][j]);
+            o.store(y + row * d + e);
         }
         if (t == 0) {
             if (mean) mean[row] = mu;
@@ -186,60 +236,60 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Rows of x and dy that are under way for each group: stages of a ring in
-// shared memory, as many as two blocks an SM (one, of rows of 32 values a thread)
-// have room for.  A thread copies and reads its own pieces only, so its
-// cp.async groups are all the synchronisation there is.
-template <typename T, int N>
+// shared memory, as many as the blocks of an SM have room for.  A thread copies
+// and reads its own pieces only, so its cp.async groups are all the
+// synchronisation there is.
+template <typename T, int GROUP, int N>
 __host__ __device__ constexpr int ring_stages() {
-    constexpr int bytes = kThreads * 2 * N * (int)sizeof(T);
-    constexpr int n = (N * (int)sizeof(T) > 64 ? 196608 : 98304) / bytes;
+    constexpr int bytes = threads_of(GROUP) * 2 * N * (int)sizeof(T);
+    constexpr int n = (threads_of(GROUP) * N * (int)sizeof(T) > 16384 ? 196608 : 98304) / bytes;
     return n > 4 ? 4 : n;
 }
 template <typename T, int GROUP, int N, bool VEC>
 constexpr size_t backward_smem() {
     // the ring, or the columns where the block's groups meet at the end
-    const size_t ring = VEC ? (size_t)ring_stages<T, N>() * kThreads * 2 * N * sizeof(T) : 0;
-    const size_t columns = GROUP < kThreads ? (size_t)GROUP * N * sizeof(Acc<T>) : 0;
+    const size_t ring = VEC ? (size_t)ring_stages<T, GROUP, N>() * threads_of(GROUP) * 2 * N * sizeof(T) : 0;
+    const size_t columns = GROUP < threads_of(GROUP) ? (size_t)GROUP * N * sizeof(Acc<T>) : 0;
     return ring > columns ? ring : columns;
 }
 
 // partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows,
 // which are consecutive
 template <typename T, typename W, int GROUP, int N, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(threads_of(GROUP))
     k_layer_norm_backward(const T *__restrict__ dy, const T *__restrict__ x,
                           const Acc<T> *__restrict__ mean, const Acc<T> *__restrict__ rstd,
                           const W *__restrict__ w, int64_t rows, int64_t d, T *__restrict__ dx,
                           Acc<T> *__restrict__ partial) {
     using A = Acc<T>;
-    using H = Held<T, N, VEC>;
-    constexpr int kGroups = kThreads / GROUP, kStages = ring_stages<T, N>();
+    using P = Piece<T, VEC>;
+    constexpr int kThreads = threads_of(GROUP), kGroups = kThreads / GROUP, kPieces = N / P::kWide;
+    constexpr int kStages = ring_stages<T, GROUP, N>();
     __shared__ A smem[2][2 * (kThreads / 32)];
     extern __shared__ __align__(16) unsigned char raw[];
-    A *columns = reinterpret_cast<A *>(raw);  // [GROUP * N], after the rows
+    A *columns = reinterpret_cast<A *>(raw);       // [GROUP * N], after the rows
     uint4 *ring = reinterpret_cast<uint4 *>(raw);  // [stage][x, dy][piece][thread]
     int turn = 0;
     const int t = threadIdx.x % GROUP;
+    auto column = [&](int i) { return (t + GROUP * i) * P::kWide; };
     const int64_t begin = rows * blockIdx.x / gridDim.x, end = rows * (blockIdx.x + 1) / gridDim.x;
-    A aw[H::kPieces][H::kWide], ab[H::kPieces][H::kWide], wv[H::kPieces][H::kWide];
+    Pair<A> aw[kPieces][P::kPairs], ab[kPieces][P::kPairs], wv[kPieces][P::kPairs];
 #pragma unroll
-    for (int i = 0; i < H::kPieces; ++i) {
-        const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
+    for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-        for (int j = 0; j < H::kWide; ++j) aw[i][j] = ab[i][j] = 0, wv[i][j] = 1;
-        if (w && e < d) load_params<W, H::kWide, VEC>(w + e, wv[i]);
+        for (int j = 0; j < P::kPairs; ++j) aw[i][j] = ab[i][j] = both(A(0)), wv[i][j] = both(A(1));
+        if (w && column(i) < d) load_params<T, VEC>(w + column(i), wv[i]);
     }
     int64_t row = begin + threadIdx.x / GROUP;
     auto fetch = [&](int64_t r, int stage) {
         if constexpr (VEC) {
             if (r < end)
 #pragma unroll
-                for (int i = 0; i < H::kPieces; ++i) {
-                    const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
-                    if (e >= d) continue;
-                    uint4 *slot = ring + ((stage * 2) * H::kPieces + i) * kThreads + threadIdx.x;
-                    cp_async<16>(smem_addr(slot), x + r * d + e);
-                    cp_async<16>(smem_addr(slot + H::kPieces * kThreads), dy + r * d + e);
+                for (int i = 0; i < kPieces; ++i) {
+                    if (column(i) >= d) continue;
+                    uint4 *slot = ring + ((stage * 2) * kPieces + i) * kThreads + threadIdx.x;
+                    cp_async<16>(smem_addr(slot), x + r * d + column(i));
+                    cp_async<16>(smem_addr(slot + kPieces * kThreads), dy + r * d + column(i));
                 }
             cp_async_commit();  // an empty group where there is no row: the count stays
         }
@@ -250,53 +300,53 @@ __global__ void __launch_bounds__(kThreads)
     A next_mu = row < end ? mean[row] : A(0), next_rs = row < end ? rstd[row] : A(0);
     for (int64_t r0 = begin; r0 < end; r0 += kGroups, row += kGroups) {
         const bool live = row < end;
-        H hx, hg;
+        P hx[kPieces], hg[kPieces];
         if constexpr (VEC) {
             // into the stage that was read last time
             fetch(row + (kStages - 1) * kGroups, stage == 0 ? kStages - 1 : stage - 1);
             cp_async_wait<kStages - 1>();
 #pragma unroll
-            for (int i = 0; i < H::kPieces; ++i) {
-                const uint4 *slot = ring + ((stage * 2) * H::kPieces + i) * kThreads + threadIdx.x;
-                hx.p[i].raw = slot[0];
-                hg.p[i].raw = slot[H::kPieces * kThreads];
+            for (int i = 0; i < kPieces; ++i) {
+                const uint4 *slot = ring + ((stage * 2) * kPieces + i) * kThreads + threadIdx.x;
+                hx[i].raw = slot[0];
+                hg[i].raw = slot[kPieces * kThreads];
             }
             stage = stage == kStages - 1 ? 0 : stage + 1;
         } else if (live) {
-            hx.template load<GROUP>(x + row * d, t, d);
-            hg.template load<GROUP>(dy + row * d, t, d);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                if (column(i) < d) hx[i].load(x + row * d + column(i)), hg[i].load(dy + row * d + column(i));
         }
-        const A mu = next_mu, rs = next_rs;
+        const Pair<A> mu = both(-next_mu), rs = both(next_rs);
         if (row + kGroups < end) next_mu = mean[row + kGroups], next_rs = rstd[row + kGroups];
-        A s1 = 0, s2 = 0;
+        Pair<A> s1 = both(A(0)), s2 = both(A(0));
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            if ((int64_t)(t + GROUP * i) * H::kWide >= d || !live) continue;
+        for (int i = 0; i < kPieces; ++i) {
+            if (column(i) >= d || !live) continue;
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) {
-                const A g = hg.at(i, j), xhat = (hx.at(i, j) - mu) * rs, v = g * wv[i][j];
-                aw[i][j] += g * xhat;
-                ab[i][j] += g;
-                s1 += v;
-                s2 += v * xhat;
+            for (int j = 0; j < P::kPairs; ++j) {
+                const Pair<A> g = hg[i].get(j), xhat = (hx[i].get(j) + mu) * rs, v = g * wv[i][j];
+                aw[i][j] = fma(g, xhat, aw[i][j]);
+                ab[i][j] = ab[i][j] + g;
+                s1 = s1 + v;
+                s2 = fma(v, xhat, s2);
             }
         }
-        group_sums<GROUP>(s1, s2, smem, turn);
-        s1 /= A(d);
-        s2 /= A(d);
+        A sums[2] = {s1.x + s1.y, s2.x + s2.y};
+        group_sums<GROUP>(sums, smem, turn);
+        s1 = both(-sums[0] / A(d));
+        s2 = both(-sums[1] / A(d));
         if (!live || !dx) continue;
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
-            if (e >= d) continue;
-            typename H::Piece o;
+        for (int i = 0; i < kPieces; ++i) {
+            if (column(i) >= d) continue;
+            P o;
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j) {
-                const A xhat = (hx.at(i, j) - mu) * rs;
-                o.v[j] = from_acc<T>(rs * (hg.at(i, j) * wv[i][j] - s1 - xhat * s2));
+            for (int j = 0; j < P::kPairs; ++j) {
+                const Pair<A> xhat = (hx[i].get(j) + mu) * rs;
+                o.set(j, rs * fma(xhat, s2, fma(hg[i].get(j), wv[i][j], s1)));
             }
-            if constexpr (VEC) __stcs(reinterpret_cast<uint4 *>(dx + row * d + e), o.raw);
-            else dx[row * d + e] = o.v[0];
+            o.store(dx + row * d + column(i));
         }
     }
     if constexpr (VEC) cp_async_wait<0>();
@@ -304,29 +354,35 @@ __global__ void __launch_bounds__(kThreads)
     // the block's groups one after the other, then the block's row of partials
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        A(&a)[H::kPieces][H::kWide] = which ? ab : aw;
+        Pair<A>(&a)[kPieces][P::kPairs] = which ? ab : aw;
         if constexpr (kGroups > 1) {
             for (int g = 0; g < kGroups; ++g) {
                 __syncthreads();
                 if (threadIdx.x / GROUP != g) continue;
 #pragma unroll
-                for (int i = 0; i < H::kPieces; ++i)
+                for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-                    for (int j = 0; j < H::kWide; ++j) {
-                        A *c = columns + (t + GROUP * i) * H::kWide + j;
-                        if (g > 0) a[i][j] += *c;
-                        *c = a[i][j];
+                    for (int j = 0; j < P::kPairs; ++j) {
+                        A *c = columns + column(i) + 2 * j;
+                        if (g > 0) a[i][j].x += c[0];
+                        c[0] = a[i][j].x;
+                        if constexpr (VEC) {
+                            if (g > 0) a[i][j].y += c[1];
+                            c[1] = a[i][j].y;
+                        }
                     }
             }
             if (threadIdx.x / GROUP != kGroups - 1) continue;
         }
         A *out = partial + (blockIdx.x * 2 + which) * d;
 #pragma unroll
-        for (int i = 0; i < H::kPieces; ++i) {
-            const int64_t e = (int64_t)(t + GROUP * i) * H::kWide;
+        for (int i = 0; i < kPieces; ++i) {
+            if (column(i) >= d) continue;
 #pragma unroll
-            for (int j = 0; j < H::kWide; ++j)
-                if (e + j < d) out[e + j] = a[i][j];
+            for (int j = 0; j < P::kPairs; ++j) {
+                out[column(i) + 2 * j] = a[i][j].x;
+                if constexpr (VEC) out[column(i) + 2 * j + 1] = a[i][j].y;
+            }
         }
     }
 }
@@ -451,28 +507,30 @@ int64_t split_rows_of(int64_t rows) {
 }
 int64_t splits_of(int64_t rows) { return (rows + split_rows_of(rows) - 1) / split_rows_of(rows); }
 
-// How a row is held: GROUP threads of N values.  Small rows take a warp, so that
-// a block works on eight; 16 values a thread (8 of 8 bytes) keep enough bytes in
-// flight with the fewest barriers.
+// How a row is held: a group of threads of 8 or 16 (float64: 8) values each.  The
+// fewest threads that hold it: what a row costs beside its values (reductions,
+// barriers, addresses) is counted in warps.  16384 x 4096 bf16 backward: 92 us
+// with 256 threads of 16, 109 us with 512 of 8 (before the packed arithmetic).
 struct Shape {
     int group, values;
 };
 Shape shape_of(int64_t d, int dtype) {
     const int most = dtype == BGL_F64 ? 8 : 16;
+    if (d <= 8 * 8) return {8, 8};
+    if (d <= 16 * 8) return {16, 8};
     if (d <= 32 * 8) return {32, 8};
-    if (d <= 32 * most) return {32, most};
-    if (d <= 128 * 8) return {128, 8};
-    if (d <= 256 * 8) return {256, 8};
-    if (d <= 256 * most) return {256, most};
-    return {256, 2 * most};
+    int group = 32;
+    while ((int64_t)group * most < d) group *= 2;
+    return {group, most};
 }
 int64_t most_held(int dtype) { return dtype == BGL_F64 ? kMostHeld / 2 : kMostHeld; }
 
 // Blocks of the backward pass, one partial row each: resident ones, a fixed
 // number for a given device so that the sums keep their order.
 int64_t backward_blocks(int64_t rows, int64_t d, int dtype) {
-    const int groups = kThreads / shape_of(d, dtype).group;
-    const int64_t want = (rows + groups - 1) / groups, most = (int64_t)num_sms() * 2;
+    const int group = shape_of(d, dtype).group, groups = threads_of(group) / group;
+    const int resident = group > kThreads ? 1 : 2;
+    const int64_t want = (rows + groups - 1) / groups, most = (int64_t)num_sms() * resident;
     return want < most ? want : most;
 }
 int64_t parts_of(int64_t rows, int64_t d, int dtype) {
@@ -496,11 +554,13 @@ struct Constant {
 template <typename T, typename F>
 int with_shape(Shape s, F &&f) {
     constexpr int M = sizeof(T) == 8 ? 8 : 16;
+    if (s.group == 8) return f(Constant<8, 8>());
+    if (s.group == 16) return f(Constant<16, 8>());
     if (s.group == 32) return s.values == 8 ? f(Constant<32, 8>()) : f(Constant<32, M>());
-    if (s.group == 128) return f(Constant<128, 8>());
-    if (s.values == 8) return f(Constant<256, 8>());
-    if (s.values == M) return f(Constant<256, M>());
-    return f(Constant<256, 2 * M>());
+    if (s.group == 64) return f(Constant<64, M>());
+    if (s.group == 128) return f(Constant<128, M>());
+    if (s.group == 256) return f(Constant<256, M>());
+    return f(Constant<512, M>());
 }
 
 struct Forward {
@@ -527,13 +587,13 @@ int forward(const Forward &p) {
     }
     const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(w, 16) && aligned(b, 16);
     return with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
-        constexpr int G = decltype(c)::group, N = decltype(c)::values, per = kThreads / G;
-        const int64_t want = (p.rows + per - 1) / per, cap = (int64_t)num_sms() * 6;
+        constexpr int G = decltype(c)::group, N = decltype(c)::values, threads = threads_of(G), per = threads / G;
+        const int64_t want = (p.rows + per - 1) / per, cap = (int64_t)num_sms() * (1536 / threads);
         const unsigned grid = (unsigned)(want < cap ? want : cap);
         if (vec)
-            k_layer_norm<T, W, G, N, true><<<grid, kThreads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+            k_layer_norm<T, W, G, N, true><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
         else
-            k_layer_norm<T, W, G, N, false><<<grid, kThreads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+            k_layer_norm<T, W, G, N, false><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
         BGL_LAUNCH_CHECK();
         return (int)BGL_OK;
     });
@@ -573,16 +633,16 @@ int backward(const Backward &p) {
     } else if (p.rows && (dx || sums)) {
         const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) && aligned(w, 16);
         const int rc = with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
-            constexpr int G = decltype(c)::group, N = decltype(c)::values;
+            constexpr int G = decltype(c)::group, N = decltype(c)::values, threads = threads_of(G);
             const unsigned grid = (unsigned)parts;
             constexpr size_t smem = backward_smem<T, G, N, true>(), plain = backward_smem<T, G, N, false>();
             if (vec) {
                 if (smem > 48 * 1024)
                     BGL_CUDA(cudaFuncSetAttribute(k_layer_norm_backward<T, W, G, N, true>,
                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-                k_layer_norm_backward<T, W, G, N, true><<<grid, kThreads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
+                k_layer_norm_backward<T, W, G, N, true><<<grid, threads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
             } else {
-                k_layer_norm_backward<T, W, G, N, false><<<grid, kThreads, plain, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
+                k_layer_norm_backward<T, W, G, N, false><<<grid, threads, plain, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
             }
             BGL_LAUNCH_CHECK();
             return (int)BGL_OK;
