@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
     const int t = threadIdx.x % GROUP;
     auto column = [&](int i) { return (t + GROUP * i) * P::kWide; };
     const int64_t stride = (int64_t)gridDim.x * kGroups, first = (int64_t)blockIdx.x * kGroups;
+    const A inv = A(1) / A(d);
     P next[kPieces];
     int64_t row = first + threadIdx.x / GROUP;
     auto fetch = [&](int64_t r) {
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         fetch(row + stride);
         A sum[1] = {s.x + s.y};
         group_sums<GROUP>(sum, smem, turn);
-        const A mu = sum[0] / A(d);
+        const A mu = sum[0] * inv;
         s = both(A(0));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         }
         sum[0] = s.x + s.y;
         group_sums<GROUP>(sum, smem, turn);
-        const A rs = A(1) / sqrt(sum[0] / A(d) + eps);
+        const A rs = A(1) / sqrt(sum[0] * inv + eps);
         if (row >= rows) continue;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
@@ -280,45 +281,55 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         for (int j = 0; j < P::kPairs; ++j) aw[i][j] = ab[i][j] = both(A(0)), wv[i][j] = both(A(1));
         if (w && column(i) < d) load_params<T, VEC>(w + column(i), wv[i]);
     }
-    int64_t row = begin + threadIdx.x / GROUP;
-    auto fetch = [&](int64_t r, int stage) {
+    // this thread's first value in its next row to fetch, and in the row at hand
+    const int64_t mine = begin + threadIdx.x / GROUP, step = kGroups * d;
+    const int count = (int)(end - begin), lead = (int)(threadIdx.x / GROUP);
+    int64_t fetched = mine * d + t * P::kWide, at = fetched;
+    constexpr uint32_t kStageBytes = 2 * kPieces * kThreads * 16, kRing = kStages * kStageBytes;
+    const uint32_t slot0 = smem_addr(ring + threadIdx.x);
+    uint32_t into = 0, from = 0;  // bytes into the ring
+    auto fetch = [&](int i_row) {
         if constexpr (VEC) {
-            if (r < end)
+            if (i_row < count)
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
                     if (column(i) >= d) continue;
-                    uint4 *slot = ring + ((stage * 2) * kPieces + i) * kThreads + threadIdx.x;
-                    cp_async<16>(smem_addr(slot), x + r * d + column(i));
-                    cp_async<16>(smem_addr(slot + kPieces * kThreads), dy + r * d + column(i));
+                    const uint32_t slot = slot0 + into + i * kThreads * 16;
+                    cp_async<16>(slot, x + fetched + GROUP * i * P::kWide);
+                    cp_async<16>(slot + kPieces * kThreads * 16, dy + fetched + GROUP * i * P::kWide);
                 }
             cp_async_commit();  // an empty group where there is no row: the count stays
+            fetched += step;
+            into = into == kRing - kStageBytes ? 0 : into + kStageBytes;
         }
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(row + i * kGroups, i);
-    int stage = 0;
-    A next_mu = row < end ? mean[row] : A(0), next_rs = row < end ? rstd[row] : A(0);
-    for (int64_t r0 = begin; r0 < end; r0 += kGroups, row += kGroups) {
-        const bool live = row < end;
+    for (int i = 0; i < kStages - 1; ++i) fetch(lead + i * kGroups);
+    const A *mu_at = mean + mine, *rs_at = rstd + mine;
+    const A inv = A(1) / A(d);
+    A next_mu = lead < count ? *mu_at : A(0), next_rs = lead < count ? *rs_at : A(0);
+    for (int r0 = 0; r0 < count; r0 += kGroups, at += step) {
+        const bool live = r0 + lead < count;
         P hx[kPieces], hg[kPieces];
         if constexpr (VEC) {
-            // into the stage that was read last time
-            fetch(row + (kStages - 1) * kGroups, stage == 0 ? kStages - 1 : stage - 1);
+            fetch(r0 + lead + (kStages - 1) * kGroups);  // into the stage that was read last time
             cp_async_wait<kStages - 1>();
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const uint4 *slot = ring + ((stage * 2) * kPieces + i) * kThreads + threadIdx.x;
+                const uint4 *slot = ring + from / 16 + i * kThreads + threadIdx.x;
                 hx[i].raw = slot[0];
                 hg[i].raw = slot[kPieces * kThreads];
             }
-            stage = stage == kStages - 1 ? 0 : stage + 1;
+            from = from == kRing - kStageBytes ? 0 : from + kStageBytes;
         } else if (live) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                if (column(i) < d) hx[i].load(x + row * d + column(i)), hg[i].load(dy + row * d + column(i));
+                if (column(i) < d)
+                    hx[i].load(x + at + GROUP * i * P::kWide), hg[i].load(dy + at + GROUP * i * P::kWide);
         }
         const Pair<A> mu = both(-next_mu), rs = both(next_rs);
-        if (row + kGroups < end) next_mu = mean[row + kGroups], next_rs = rstd[row + kGroups];
+        mu_at += kGroups, rs_at += kGroups;
+        if (r0 + lead + kGroups < count) next_mu = *mu_at, next_rs = *rs_at;
         Pair<A> s1 = both(A(0)), s2 = both(A(0));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
@@ -334,8 +345,8 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         }
         A sums[2] = {s1.x + s1.y, s2.x + s2.y};
         group_sums<GROUP>(sums, smem, turn);
-        s1 = both(-sums[0] / A(d));
-        s2 = both(-sums[1] / A(d));
+        s1 = both(-sums[0] * inv);
+        s2 = both(-sums[1] * inv);
         if (!live || !dx) continue;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
@@ -346,7 +357,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
                 const Pair<A> xhat = (hx[i].get(j) + mu) * rs;
                 o.set(j, rs * fma(xhat, s2, fma(hg[i].get(j), wv[i][j], s1)));
             }
-            o.store(dx + row * d + column(i));
+            o.store(dx + at + GROUP * i * P::kWide);
         }
     }
     if constexpr (VEC) cp_async_wait<0>();
