@@ -69,33 +69,38 @@ __device__ __forceinline__ Pair<double> fma(Pair<double> a, Pair<double> b, Pair
 template <typename A>
 __device__ __forceinline__ Pair<A> both(A v) { return {v, v}; }
 
-// Values of a row as they are in memory: pieces of 16 bytes (VEC), or of one
-// value whose pair partner is zero.
+// Values of a row as they are in memory: pieces of 16 bytes (VEC), or of two
+// values that are moved one by one; the second one of a row's last piece may lie
+// behind the row (`left` values remain), and is zero then.
 template <typename T, bool VEC>
 struct Piece {
-    static constexpr int kWide = VEC ? 16 / (int)sizeof(T) : 1;
-    static constexpr int kPairs = VEC ? kWide / 2 : 1;
+    static constexpr int kWide = VEC ? 16 / (int)sizeof(T) : 2;
+    static constexpr int kPairs = kWide / 2;
     union {
         uint4 raw;
-        T v[VEC ? kWide : 1];
+        T v[kWide];
     };
     __device__ Piece() {}
 
-    __device__ __forceinline__ void load(const T *p) {
-        if constexpr (VEC) raw = __ldcs(reinterpret_cast<const uint4 *>(p));
-        else v[0] = *p;
+    __device__ __forceinline__ void load(const T *p, int64_t left) {
+        if constexpr (VEC) {
+            raw = __ldcs(reinterpret_cast<const uint4 *>(p));
+        } else {
+            v[0] = p[0];
+            v[1] = left > 1 ? p[1] : from_acc<T>(0);
+        }
     }
-    __device__ __forceinline__ void store(T *p) const {
-        if constexpr (VEC) __stcs(reinterpret_cast<uint4 *>(p), raw);
-        else *p = v[0];
+    __device__ __forceinline__ void store(T *p, int64_t left) const {
+        if constexpr (VEC) {
+            __stcs(reinterpret_cast<uint4 *>(p), raw);
+        } else {
+            p[0] = v[0];
+            if (left > 1) p[1] = v[1];
+        }
     }
-    __device__ __forceinline__ Pair<Acc<T>> get(int i) const {
-        if constexpr (VEC) return {to_acc(v[2 * i]), to_acc(v[2 * i + 1])};
-        else return {to_acc(v[0]), Acc<T>(0)};
-    }
+    __device__ __forceinline__ Pair<Acc<T>> get(int i) const { return {to_acc(v[2 * i]), to_acc(v[2 * i + 1])}; }
     __device__ __forceinline__ void set(int i, Pair<Acc<T>> p) {
-        if constexpr (VEC) v[2 * i] = from_acc<T>(p.x), v[2 * i + 1] = from_acc<T>(p.y);
-        else v[0] = from_acc<T>(p.x);
+        v[2 * i] = from_acc<T>(p.x), v[2 * i + 1] = from_acc<T>(p.y);
     }
 };
 template <>
@@ -105,7 +110,7 @@ __device__ __forceinline__ void Piece<__nv_bfloat16, true>::set(int i, Pair<floa
 
 // The parameters of a piece at p, in 16-byte loads where VEC.
 template <typename T, bool VEC, typename W>
-__device__ __forceinline__ void load_params(const W *p, Pair<Acc<T>> (&v)[Piece<T, VEC>::kPairs]) {
+__device__ __forceinline__ void load_params(const W *p, int64_t left, Pair<Acc<T>> (&v)[Piece<T, VEC>::kPairs]) {
     using A = Acc<T>;
     if constexpr (VEC) {
         constexpr int kWide = 16 / (int)sizeof(W), kLoads = Piece<T, true>::kWide / kWide;
@@ -121,7 +126,7 @@ __device__ __forceinline__ void load_params(const W *p, Pair<Acc<T>> (&v)[Piece<
                 v[i * (kWide / 2) + j] = {A(to_acc(u.w[2 * j])), A(to_acc(u.w[2 * j + 1]))};
         }
     } else {
-        v[0] = {A(to_acc(*p)), A(0)};
+        v[0] = {A(to_acc(p[0])), left > 1 ? A(to_acc(p[1])) : A(0)};
     }
 }
 
@@ -154,8 +159,13 @@ __device__ __forceinline__ void group_sums(A (&v)[K], A (*smem)[K * (threads_of(
     }
 }
 
+// Blocks an SM that the forward pass is compiled for, and the grid filled with.
+__host__ __device__ constexpr int forward_resident(int group, int values, int size) {
+    return (size == 8 ? 3 : values == 8 ? 5 : 4) * kThreads / threads_of(group);
+}
+
 template <typename T, typename W, int GROUP, int N, bool VEC>
-__global__ void __launch_bounds__(threads_of(GROUP))
+__global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, sizeof(T)))
     k_layer_norm(const T *__restrict__ x, const W *__restrict__ w, const W *__restrict__ b,
                  int64_t rows, int64_t d, Acc<T> eps, T *__restrict__ y, Acc<T> *__restrict__ mean,
                  Acc<T> *__restrict__ rstd) {
@@ -174,7 +184,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         if (r < rows)
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                if (column(i) < d) next[i].load(x + r * d + column(i));
+                if (column(i) < d) next[i].load(x + r * d + column(i), d - column(i));
     };
     fetch(row);
     // whole groups take part in the block's barriers even behind the last row
@@ -200,7 +210,8 @@ __global__ void __launch_bounds__(threads_of(GROUP))
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
                 v[i][j] = v[i][j] + both(-mu);
-                if (column(i) < d) s = VEC ? fma(v[i][j], v[i][j], s) : Pair<A>{s.x + v[i][j].x * v[i][j].x, 0};
+                if (!VEC && column(i) + 1 >= d) v[i][j].y = 0;
+                if (column(i) < d) s = fma(v[i][j], v[i][j], s);
             }
         }
         sum[0] = s.x + s.y;
@@ -215,25 +226,32 @@ __global__ void __launch_bounds__(threads_of(GROUP))
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * both(rs);
             if (w) {
-                load_params<T, VEC>(w + e, p);
+                load_params<T, VEC>(w + e, d - e, p);
 #pragma unroll
                 for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * p[j];
             }
             if (b) {
-                load_params<T, VEC>(b + e, p);
+                load_params<T, VEC>(b + e, d - e, p);
 #pragma unroll
                 for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] + p[j];
             }
             P o;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) o.set(j, v[i][j]);
-            o.store(y + row * d + e);
+            o.store(y + row * d + e, d - e);
         }
         if (t == 0) {
             if (mean) mean[row] = mu;
             if (rstd) rstd[row] = rs;
         }
     }
+}
+
+// Blocks an SM that the backward pass is compiled for: what its registers allow
+// without spills (16384 x 4096 bf16: 89 us with two, 100 us with three; 131072 x
+// 256: 54 us with two, 49 us with three).
+__host__ __device__ constexpr int backward_resident(int group, int values, int size) {
+    return group > kThreads || size == 8 ? 1 : values == 8 && size == 2 ? 3 : 2;
 }
 
 // Rows of x and dy that are under way for each group: stages of a ring in
@@ -243,7 +261,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
 template <typename T, int GROUP, int N>
 __host__ __device__ constexpr int ring_stages() {
     constexpr int bytes = threads_of(GROUP) * 2 * N * (int)sizeof(T);
-    constexpr int n = (threads_of(GROUP) * N * (int)sizeof(T) > 16384 ? 196608 : 98304) / bytes;
+    constexpr int n = 196608 / backward_resident(GROUP, N, sizeof(T)) / bytes;
     return n > 4 ? 4 : n;
 }
 template <typename T, int GROUP, int N, bool VEC>
@@ -257,7 +275,7 @@ constexpr size_t backward_smem() {
 // partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows,
 // which are consecutive
 template <typename T, typename W, int GROUP, int N, bool VEC>
-__global__ void __launch_bounds__(threads_of(GROUP))
+__global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N, sizeof(T)))
     k_layer_norm_backward(const T *__restrict__ dy, const T *__restrict__ x,
                           const Acc<T> *__restrict__ mean, const Acc<T> *__restrict__ rstd,
                           const W *__restrict__ w, int64_t rows, int64_t d, T *__restrict__ dx,
@@ -279,7 +297,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
     for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
         for (int j = 0; j < P::kPairs; ++j) aw[i][j] = ab[i][j] = both(A(0)), wv[i][j] = both(A(1));
-        if (w && column(i) < d) load_params<T, VEC>(w + column(i), wv[i]);
+        if (w && column(i) < d) load_params<T, VEC>(w + column(i), d - column(i), wv[i]);
     }
     // this thread's first value in its next row to fetch, and in the row at hand
     const int64_t mine = begin + threadIdx.x / GROUP, step = kGroups * d;
@@ -324,23 +342,31 @@ __global__ void __launch_bounds__(threads_of(GROUP))
         } else if (live) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                if (column(i) < d)
-                    hx[i].load(x + at + GROUP * i * P::kWide), hg[i].load(dy + at + GROUP * i * P::kWide);
+                if (column(i) < d) {
+                    hx[i].load(x + at + GROUP * i * P::kWide, d - column(i));
+                    hg[i].load(dy + at + GROUP * i * P::kWide, d - column(i));
+                }
         }
         const Pair<A> mu = both(-next_mu), rs = both(next_rs);
         mu_at += kGroups, rs_at += kGroups;
         if (r0 + lead + kGroups < count) next_mu = *mu_at, next_rs = *rs_at;
         Pair<A> s1 = both(A(0)), s2 = both(A(0));
+        // bf16: kept as they are worked out (unpacking them again costs more
+        // than the registers); else worked out again
+        constexpr bool kKeep = sizeof(T) == 2;
+        Pair<A> xhat[kPieces][P::kPairs], v[kPieces][P::kPairs];
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             if (column(i) >= d || !live) continue;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
-                const Pair<A> g = hg[i].get(j), xhat = (hx[i].get(j) + mu) * rs, v = g * wv[i][j];
-                aw[i][j] = fma(g, xhat, aw[i][j]);
+                const Pair<A> g = hg[i].get(j);
+                xhat[i][j] = (hx[i].get(j) + mu) * rs;
+                v[i][j] = g * wv[i][j];
+                aw[i][j] = fma(g, xhat[i][j], aw[i][j]);
                 ab[i][j] = ab[i][j] + g;
-                s1 = s1 + v;
-                s2 = fma(v, xhat, s2);
+                s1 = s1 + v[i][j];
+                s2 = fma(v[i][j], xhat[i][j], s2);
             }
         }
         A sums[2] = {s1.x + s1.y, s2.x + s2.y};
@@ -354,10 +380,13 @@ __global__ void __launch_bounds__(threads_of(GROUP))
             P o;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
-                const Pair<A> xhat = (hx[i].get(j) + mu) * rs;
-                o.set(j, rs * fma(xhat, s2, fma(hg[i].get(j), wv[i][j], s1)));
+                if constexpr (!kKeep) {
+                    xhat[i][j] = (hx[i].get(j) + mu) * rs;
+                    v[i][j] = hg[i].get(j) * wv[i][j];
+                }
+                o.set(j, rs * fma(xhat[i][j], s2, v[i][j] + s1));
             }
-            o.store(dx + at + GROUP * i * P::kWide);
+            o.store(dx + at + GROUP * i * P::kWide, d - column(i));
         }
     }
     if constexpr (VEC) cp_async_wait<0>();
@@ -377,10 +406,8 @@ __global__ void __launch_bounds__(threads_of(GROUP))
                         A *c = columns + column(i) + 2 * j;
                         if (g > 0) a[i][j].x += c[0];
                         c[0] = a[i][j].x;
-                        if constexpr (VEC) {
-                            if (g > 0) a[i][j].y += c[1];
-                            c[1] = a[i][j].y;
-                        }
+                        if (g > 0) a[i][j].y += c[1];
+                        c[1] = a[i][j].y;
                     }
             }
             if (threadIdx.x / GROUP != kGroups - 1) continue;
@@ -392,7 +419,7 @@ __global__ void __launch_bounds__(threads_of(GROUP))
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
                 out[column(i) + 2 * j] = a[i][j].x;
-                if constexpr (VEC) out[column(i) + 2 * j + 1] = a[i][j].y;
+                if (VEC || column(i) + 1 < d) out[column(i) + 2 * j + 1] = a[i][j].y;
             }
         }
     }
@@ -539,8 +566,9 @@ int64_t most_held(int dtype) { return dtype == BGL_F64 ? kMostHeld / 2 : kMostHe
 // Blocks of the backward pass, one partial row each: resident ones, a fixed
 // number for a given device so that the sums keep their order.
 int64_t backward_blocks(int64_t rows, int64_t d, int dtype) {
-    const int group = shape_of(d, dtype).group, groups = threads_of(group) / group;
-    const int resident = group > kThreads ? 1 : 2;
+    const Shape shape = shape_of(d, dtype);
+    const int groups = threads_of(shape.group) / shape.group;
+    const int resident = backward_resident(shape.group, shape.values, (int)row_elem_size(dtype));
     const int64_t want = (rows + groups - 1) / groups, most = (int64_t)num_sms() * resident;
     return want < most ? want : most;
 }
@@ -599,7 +627,9 @@ int forward(const Forward &p) {
     const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(w, 16) && aligned(b, 16);
     return with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
         constexpr int G = decltype(c)::group, N = decltype(c)::values, threads = threads_of(G), per = threads / G;
-        const int64_t want = (p.rows + per - 1) / per, cap = (int64_t)num_sms() * (1536 / threads);
+        // one wave of resident blocks (888 blocks where 592 are resident: 38 us
+        // for 8192 x 4096 bf16, against 33 us)
+        const int64_t want = (p.rows + per - 1) / per, cap = (int64_t)num_sms() * forward_resident(G, N, sizeof(T));
         const unsigned grid = (unsigned)(want < cap ? want : cap);
         if (vec)
             k_layer_norm<T, W, G, N, true><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
