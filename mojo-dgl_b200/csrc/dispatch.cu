@@ -9,94 +9,155 @@
 //
 //   dispatch:  rows[p] = x[t]                     combine:  y[t] = sum_j w[t, j] rows[p]
 //   backward:  drows[p] = w[t, j] dy[t],  dw[t, j] = <dy[t], rows[p]>     (p = positions[t, j])
+//
+// Memory bounds the three of them: each reads a token's row once for its k
+// choices, in 16-byte pieces where the row length and the addresses allow, the
+// lanes of a token side by side over its row.
 #include "rows.cuh"
 
 namespace bgl {
 namespace {
 
-constexpr int kMaxBins = 8192;   // experts + 1: one shared-memory counter each
+constexpr int kThreads = 256;
+constexpr int kMaxBins = 8192;           // experts + 1: shared-memory counters
+constexpr int kCounters = 48 * 1024 / 4; // of a block
 constexpr int kMaxChunks = 2048;
 
+// ---------------------------------------------------------------- the plan
 // Item i's bin: its expert, or `experts` (the last bin) for none.
 __device__ __forceinline__ int bin_of(int64_t index, int experts) {
     return index >= 0 && index < experts ? (int)index : experts;
 }
 
-int64_t chunk_items(int64_t items) {
-    int64_t per = (items + kMaxChunks - 1) / kMaxChunks;
-    if (per < 1024) per = 1024;
-    return (per + 31) / 32 * 32;
+// A chunk of consecutive items goes to one block, an equal part of it to each of
+// its warps, which counts and ranks 32 items a step.  As many warps as the
+// counters of all of them leave room for.
+struct Plan {
+    int64_t items, chunks, per_warp;
+    int experts, warps;
+};
+Plan plan_of(int64_t items, int64_t experts) {
+    Plan p;
+    p.items = items;
+    p.experts = (int)experts;
+    const int64_t room = kCounters / (experts + 1);
+    p.warps = (int)(room < 8 ? room : 8);
+    // 256 items a warp, more where that gave too many chunks; one chunk where 32
+    // steps a warp are enough (one launch instead of three)
+    int64_t steps = (items + p.warps * 32 * (int64_t)kMaxChunks - 1) / (p.warps * 32 * (int64_t)kMaxChunks);
+    if (steps < 8) steps = 8;
+    if (items <= p.warps * 32 * 32) steps = (items + p.warps * 32 - 1) / (p.warps * 32);
+    p.per_warp = (steps > 0 ? steps : 1) * 32;
+    p.chunks = (items + p.per_warp * p.warps - 1) / (p.per_warp * p.warps);
+    return p;
 }
-int64_t num_chunks(int64_t items) { return (items + chunk_items(items) - 1) / chunk_items(items); }
 
-// bins of one chunk of consecutive items
-__global__ void __launch_bounds__(256)
-    k_plan_count(const int64_t *__restrict__ indices, int64_t items, int64_t per, int experts,
-                 int32_t *__restrict__ chunk_bins) {
+// chunk_bins[bin][chunk] = items of the chunk in the bin
+__global__ void __launch_bounds__(kThreads)
+    k_plan_count(const Plan p, const int64_t *__restrict__ indices, int32_t *__restrict__ chunk_bins) {
     extern __shared__ int32_t bins[];
-    for (int b = threadIdx.x; b <= experts; b += blockDim.x) bins[b] = 0;
+    for (int b = threadIdx.x; b <= p.experts; b += blockDim.x) bins[b] = 0;
     __syncthreads();
-    const int64_t i0 = blockIdx.x * per, i1 = i0 + per < items ? i0 + per : items;
+    const int64_t per = p.per_warp * p.warps, i0 = blockIdx.x * per;
+    const int64_t i1 = i0 + per < p.items ? i0 + per : p.items;
     for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x)
-        atomicAdd(&bins[bin_of(indices[i], experts)], 1);
+        atomicAdd(&bins[bin_of(indices[i], p.experts)], 1);
     __syncthreads();
-    for (int b = threadIdx.x; b <= experts; b += blockDim.x)
-        chunk_bins[blockIdx.x * (int64_t)(experts + 1) + b] = bins[b];
+    for (int b = threadIdx.x; b <= p.experts; b += blockDim.x)
+        chunk_bins[b * p.chunks + blockIdx.x] = bins[b];
 }
 
-// chunk_bins becomes the first row of each (chunk, bin); one block
-__global__ void __launch_bounds__(1024)
-    k_plan_scan(int32_t *__restrict__ chunk_bins, int64_t chunks, int experts,
+// In place, for each bin the items in earlier chunks; the bin's total behind them.  A warp a bin.
+__global__ void __launch_bounds__(kThreads)
+    k_plan_scan(const Plan p, int32_t *__restrict__ chunk_bins, int32_t *__restrict__ totals,
                 int64_t *__restrict__ counts) {
-    extern __shared__ int32_t total[];
-    for (int b = threadIdx.x; b <= experts; b += blockDim.x) {
-        int32_t sum = 0;
-        for (int64_t c = 0; c < chunks; ++c) {
-            int32_t *p = chunk_bins + c * (experts + 1) + b;
-            const int32_t n = *p;
-            *p = sum;
-            sum += n;
+    const int lane = threadIdx.x & 31, bin = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (bin > p.experts) return;
+    int32_t sum = 0;
+    for (int64_t c0 = 0; c0 < p.chunks; c0 += 32) {
+        int32_t *at = chunk_bins + bin * p.chunks + c0 + lane;
+        const int32_t n = c0 + lane < p.chunks ? *at : 0;
+        int32_t scan = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += up;
         }
-        total[b] = sum;
-        if (b < experts) counts[b] = sum;
+        if (c0 + lane < p.chunks) *at = sum + scan - n;
+        sum += __shfl_sync(0xffffffffu, scan, 31);
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int32_t sum = 0;
-        for (int b = 0; b <= experts; ++b) {
-            const int32_t n = total[b];
-            total[b] = sum;
-            sum += n;
-        }
+    if (lane == 0) {
+        totals[bin] = sum;
+        if (bin < p.experts) counts[bin] = sum;
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b <= experts; b += blockDim.x)
-        for (int64_t c = 0; c < chunks; ++c) chunk_bins[c * (experts + 1) + b] += total[b];
 }
 
-// one warp a chunk, 32 items a step in order
-__global__ void __launch_bounds__(32)
-    k_plan_place(const int64_t *__restrict__ indices, int64_t items, int64_t per, int experts,
-                 const int32_t *__restrict__ chunk_bins, int32_t *__restrict__ positions) {
-    extern __shared__ int32_t next[];
-    const int lane = threadIdx.x;
-    for (int b = lane; b <= experts; b += 32)
-        next[b] = chunk_bins[blockIdx.x * (int64_t)(experts + 1) + b];
-    __syncwarp();
-    const int64_t i0 = blockIdx.x * per, i1 = i0 + per < items ? i0 + per : items;
+// Rows of a chunk's items.  With one chunk, its own counts are the totals.
+__global__ void __launch_bounds__(kThreads)
+    k_plan_place(const Plan p, const int64_t *__restrict__ indices,
+                 const int32_t *__restrict__ chunk_bins, const int32_t *__restrict__ totals,
+                 int32_t *__restrict__ positions, int64_t *__restrict__ counts) {
+    extern __shared__ int32_t next[];  // [warp][bin]
+    __shared__ int32_t warp_sums[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = p.experts + 1;
+    for (int b = threadIdx.x; b < p.warps * bins; b += blockDim.x) next[b] = 0;
+    __syncthreads();
+    int32_t *mine = next + warp * bins;
+    const int64_t i0 = (blockIdx.x * (int64_t)p.warps + warp) * p.per_warp;
+    const int64_t i1 = i0 + p.per_warp < p.items ? i0 + p.per_warp : p.items;
+#pragma unroll 4
+    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[bin_of(indices[i], p.experts)], 1);
+    __syncthreads();
+    // each bin's first row: all items of lower bins, those of its own in earlier
+    // chunks, those of this chunk's earlier warps
+    int32_t before = 0;
+    for (int b0 = 0; b0 < bins; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int32_t own = 0;
+        if (b < bins) {
+            for (int w = 0; w < p.warps; ++w) {
+                const int32_t n = next[w * bins + b];
+                next[w * bins + b] = own;
+                own += n;
+            }
+            if (p.chunks > 1) own = totals[b];
+            else if (b < p.experts) counts[b] = own;
+        }
+        int32_t scan = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t up = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += up;
+        }
+        if (lane == 31) warp_sums[warp] = scan;
+        __syncthreads();
+        int32_t all = 0, lower = 0;
+        for (int w = 0; w < p.warps; ++w) {
+            if (w < warp) lower += warp_sums[w];
+            all += warp_sums[w];
+        }
+        if (b < bins) {
+            int32_t first = before + lower + scan - own;
+            if (p.chunks > 1) first += chunk_bins[b * p.chunks + blockIdx.x];
+            for (int w = 0; w < p.warps; ++w) next[w * bins + b] += first;
+        }
+        before += all;
+        __syncthreads();
+    }
     for (int64_t i = i0; i < i1; i += 32) {
         const bool in = i + lane < i1;
-        const int bin = in ? bin_of(indices[i + lane], experts) : -1;
+        const int bin = in ? bin_of(indices[i + lane], p.experts) : -1;
         const unsigned same = __match_any_sync(0xffffffffu, bin);
-        const int before = __popc(same & ((1u << lane) - 1));
-        const int32_t p = in ? next[bin] + before : 0;
+        const int earlier = __popc(same & ((1u << lane) - 1));
+        const int32_t row = in ? mine[bin] + earlier : 0;
         __syncwarp();
-        if (in && before == 0) next[bin] += __popc(same);
+        if (in && earlier == 0) mine[bin] = row + __popc(same);
         __syncwarp();
-        if (in) positions[i + lane] = bin == experts ? ~p : p;
+        if (in) positions[i + lane] = bin == p.experts ? ~row : row;
     }
 }
 
+// -------------------------------------------------------------------- rows
 // Row of a position; false where the pair has no expert.  A position outside
 // [0, total) is not one of a plan's: it gives row -1, which is not touched.
 __device__ __forceinline__ bool row_of(int32_t position, int64_t total, int64_t &row) {
@@ -105,64 +166,146 @@ __device__ __forceinline__ bool row_of(int32_t position, int64_t total, int64_t 
     return position >= 0 && row >= 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+// Consecutive values of a row: 16 bytes, or one.
+template <typename T, bool VEC>
+struct Piece {
+    static constexpr int kWide = VEC ? 16 / (int)sizeof(T) : 1;
+    union {
+        uint4 raw;
+        T v[kWide];
+    };
+    __device__ Piece() {}
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC) raw = __ldg(reinterpret_cast<const uint4 *>(p));
+        else v[0] = *p;
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (VEC) *reinterpret_cast<uint4 *>(p) = raw;
+        else *p = v[0];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWide; ++i) v[i] = from_acc<T>(0);
+    }
+};
+
+// blockDim.x threads over a row's pieces, blockDim.y tokens.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads)
     k_dispatch(const T *__restrict__ x, const int32_t *__restrict__ positions, int64_t tokens,
                int k, int64_t d, T *__restrict__ rows) {
-    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
+    using P = Piece<T, VEC>;
+    const int64_t t = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    const int32_t *pos = positions + t * k;
+    P none;
+    none.zero();
+    for (int64_t e = threadIdx.x * P::kWide; e < d; e += blockDim.x * P::kWide) {
+        P v;
+        v.load(x + t * d + e);
+#pragma unroll 4
         for (int j = 0; j < k; ++j) {
             int64_t row;
-            const bool sent = row_of(positions[t * k + j], tokens * k, row);
-            if (row < 0) continue;
-            for (int64_t i = threadIdx.x; i < d; i += blockDim.x)
-                rows[row * d + i] = sent ? x[t * d + i] : from_acc<T>(0);
+            const bool sent = row_of(__ldg(pos + j), tokens * k, row);
+            if (row >= 0) (sent ? v : none).store(rows + row * d + e);
         }
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads)
     k_combine(const T *__restrict__ rows, const int32_t *__restrict__ positions,
               const Acc<T> *__restrict__ weights, int64_t tokens, int k, int64_t d,
               T *__restrict__ y) {
     using A = Acc<T>;
-    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-        for (int64_t i = threadIdx.x; i < d; i += blockDim.x) {
-            A sum = 0;
-            for (int j = 0; j < k; ++j) {
+    using P = Piece<T, VEC>;
+    constexpr int kFlight = 4;  // rows under way
+    const int64_t t = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    const int32_t *pos = positions + t * k;
+    for (int64_t e = threadIdx.x * P::kWide; e < d; e += blockDim.x * P::kWide) {
+        A sum[P::kWide];
+#pragma unroll
+        for (int i = 0; i < P::kWide; ++i) sum[i] = 0;
+        for (int j0 = 0; j0 < k; j0 += kFlight) {
+            P v[kFlight];
+            A w[kFlight];
+            bool sent[kFlight];
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j) {
                 int64_t row;
-                if (!row_of(positions[t * k + j], tokens * k, row)) continue;
-                const A v = to_acc(rows[row * d + i]);
-                sum += weights ? weights[t * k + j] * v : v;
+                sent[j] = j0 + j < k && row_of(__ldg(pos + j0 + j), tokens * k, row);
+                if (sent[j]) {
+                    v[j].load(rows + row * d + e);
+                    w[j] = weights ? __ldg(weights + t * k + j0 + j) : A(1);
+                }
             }
-            y[t * d + i] = from_acc<T>(sum);
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j)
+                if (sent[j])
+#pragma unroll
+                    for (int i = 0; i < P::kWide; ++i) sum[i] += w[j] * to_acc(v[j].v[i]);
         }
+        P o;
+#pragma unroll
+        for (int i = 0; i < P::kWide; ++i) o.v[i] = from_acc<T>(sum[i]);
+        o.store(y + t * d + e);
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+// GROUP threads a token, `kFlight` choices at a time: dy is read once for them.
+template <typename T, int GROUP, bool VEC>
+__global__ void __launch_bounds__(kThreads)
     k_combine_backward(const T *__restrict__ dy, const T *__restrict__ rows,
                        const int32_t *__restrict__ positions, const Acc<T> *__restrict__ weights,
                        int64_t tokens, int k, int64_t d, T *__restrict__ drows,
                        Acc<T> *__restrict__ dweights) {
     using A = Acc<T>;
+    using P = Piece<T, VEC>;
+    constexpr int kFlight = 4;
     __shared__ A smem[32];
-    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-        for (int j = 0; j < k; ++j) {
-            int64_t row;
-            const bool sent = row_of(positions[t * k + j], tokens * k, row);
-            const A w = !sent ? A(0) : weights ? weights[t * k + j] : A(1);
-            A dot = 0;
-            if (row >= 0)
-                for (int64_t i = threadIdx.x; i < d; i += blockDim.x) {
-                    const A g = sent ? to_acc(dy[t * d + i]) : A(0);
-                    if (dweights && sent) dot += g * to_acc(rows[row * d + i]);
-                    if (drows) drows[row * d + i] = from_acc<T>(w * g);
+    const int own = threadIdx.x % GROUP;
+    const int64_t t = blockIdx.x * (int64_t)(kThreads / GROUP) + threadIdx.x / GROUP;
+    if (t >= tokens) return;  // whole groups; a group of a block is the block
+    for (int j0 = 0; j0 < k; j0 += kFlight) {
+        int64_t row[kFlight];
+        bool sent[kFlight];
+        A w[kFlight], dot[kFlight];
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+            row[j] = -1;
+            sent[j] = j0 + j < k && row_of(__ldg(positions + t * k + j0 + j), tokens * k, row[j]);
+            w[j] = !sent[j] ? A(0) : weights ? __ldg(weights + t * k + j0 + j) : A(1);
+            dot[j] = 0;
+        }
+#pragma unroll 2
+        for (int64_t e = own * P::kWide; e < d; e += GROUP * P::kWide) {
+            P g, v[kFlight];
+            g.load(dy + t * d + e);
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j)
+                if (dweights && sent[j]) v[j].load(rows + row[j] * d + e);
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j) {
+                if (row[j] < 0) continue;
+                P o;
+#pragma unroll
+                for (int i = 0; i < P::kWide; ++i) {
+                    const A gi = to_acc(g.v[i]);
+                    if (dweights && sent[j]) dot[j] += gi * to_acc(v[j].v[i]);
+                    o.v[i] = from_acc<T>(sent[j] ? w[j] * gi : A(0));
                 }
-            if (dweights) {
-                dot = block_sum(dot, smem);
-                if (threadIdx.x == 0) dweights[t * k + j] = dot;
+                if (drows) o.store(drows + row[j] * d + e);
             }
         }
+        if (!dweights) continue;
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+            if (j0 + j >= k) break;
+            const A sum = GROUP == 32 ? warp_sum(dot[j]) : block_sum(dot[j], smem);
+            if (own == 0) dweights[t * k + j0 + j] = sum;
+        }
+    }
 }
 
 int check_rows(const char *who, int64_t tokens, int64_t k, int64_t d, int dtype) {
@@ -173,9 +316,68 @@ int check_rows(const char *who, int64_t tokens, int64_t k, int64_t d, int dtype)
     return BGL_OK;
 }
 
-unsigned token_blocks(int64_t tokens) {
-    const int64_t cap = (int64_t)num_sms() * 8;
-    return (unsigned)(tokens < cap ? tokens : cap);
+// Threads over a row's pieces and tokens of a block: a power of two of threads, 8
+// to 256, that no row leaves mostly idle.
+dim3 row_block(int64_t pieces) {
+    unsigned x = 8;
+    while (x < pieces && x < kThreads) x *= 2;
+    return dim3(x, kThreads / x);
+}
+template <typename T>
+bool pieces_of_16(int64_t d, const void *a, const void *b, const void *c = nullptr) {
+    return d * sizeof(T) % 16 == 0 && aligned(a, 16) && aligned(b, 16) && aligned(c, 16);
+}
+unsigned token_blocks(int64_t tokens, unsigned per) { return (unsigned)((tokens + per - 1) / per); }
+
+struct Rows {
+    const void *in, *rows;
+    const int32_t *positions;
+    const void *weights;
+    int64_t tokens, d;
+    int k;
+    void *out, *dweights;
+    cudaStream_t s;
+};
+template <typename T>
+int dispatch_as(const Rows &p) {
+    const bool vec = pieces_of_16<T>(p.d, p.in, p.out);
+    const dim3 block = row_block(vec ? p.d * (int64_t)sizeof(T) / 16 : p.d);
+    const unsigned grid = token_blocks(p.tokens, block.y);
+    if (vec) k_dispatch<T, true><<<grid, block, 0, p.s>>>((const T *)p.in, p.positions, p.tokens, p.k, p.d, (T *)p.out);
+    else k_dispatch<T, false><<<grid, block, 0, p.s>>>((const T *)p.in, p.positions, p.tokens, p.k, p.d, (T *)p.out);
+    BGL_LAUNCH_CHECK();
+    return BGL_OK;
+}
+template <typename T>
+int combine_as(const Rows &p) {
+    using A = Acc<T>;
+    const bool vec = pieces_of_16<T>(p.d, p.rows, p.out);
+    const dim3 block = row_block(vec ? p.d * (int64_t)sizeof(T) / 16 : p.d);
+    const unsigned grid = token_blocks(p.tokens, block.y);
+    const T *rows = (const T *)p.rows;
+    const A *w = (const A *)p.weights;
+    if (vec) k_combine<T, true><<<grid, block, 0, p.s>>>(rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out);
+    else k_combine<T, false><<<grid, block, 0, p.s>>>(rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out);
+    BGL_LAUNCH_CHECK();
+    return BGL_OK;
+}
+template <typename T, int GROUP>
+int combine_backward_as(const Rows &p) {
+    using A = Acc<T>;
+    const T *dy = (const T *)p.in, *rows = (const T *)p.rows;
+    const A *w = (const A *)p.weights;
+    const unsigned grid = token_blocks(p.tokens, kThreads / GROUP);
+    if (pieces_of_16<T>(p.d, p.in, p.rows, p.out))
+        k_combine_backward<T, GROUP, true><<<grid, kThreads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
+    else
+        k_combine_backward<T, GROUP, false><<<grid, kThreads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
+    BGL_LAUNCH_CHECK();
+    return BGL_OK;
+}
+template <typename T>
+int combine_backward_as(const Rows &p) {
+    // a warp a token (no barriers), a block where there are too few tokens for that
+    return p.tokens >= (int64_t)num_sms() * 16 ? combine_backward_as<T, 32>(p) : combine_backward_as<T, kThreads>(p);
 }
 
 }  // namespace
@@ -186,8 +388,9 @@ using namespace bgl;
 extern "C" {
 
 size_t bgl_expert_plan_workspace_size(int64_t items, int64_t experts) {
-    if (items < 0 || experts < 0) return 0;
-    return (size_t)num_chunks(items) * (experts + 1) * sizeof(int32_t) + 256;
+    if (items < 0 || experts < 1 || experts >= kMaxBins) return 0;
+    const Plan p = plan_of(items, experts);
+    return p.chunks > 1 ? (size_t)(p.chunks + 1) * (experts + 1) * sizeof(int32_t) + 512 : 0;
 }
 
 int bgl_expert_plan(const int64_t *indices, int64_t items, int64_t experts, int64_t *counts,
@@ -198,24 +401,25 @@ int bgl_expert_plan(const int64_t *indices, int64_t items, int64_t experts, int6
         return fail(BGL_E_UNSUPPORTED, "bgl_expert_plan: more than %d experts", kMaxBins - 1);
     if (!counts || (items && (!indices || !positions)))
         return fail(BGL_E_INVALID, "bgl_expert_plan: null buffer");
-    if (!workspace || workspace_bytes < bgl_expert_plan_workspace_size(items, experts))
+    const size_t need = bgl_expert_plan_workspace_size(items, experts);
+    if (need && (!workspace || workspace_bytes < need))
         return fail(BGL_E_WORKSPACE, "bgl_expert_plan: workspace too small");
     cudaStream_t s = as_stream(stream);
-    Carver c(workspace);
-    const int64_t chunks = num_chunks(items), per = chunk_items(items);
-    int32_t *chunk_bins = c.take<int32_t>((size_t)chunks * (experts + 1));
-    const size_t smem = (size_t)(experts + 1) * sizeof(int32_t);
-    if (chunks) {
-        k_plan_count<<<(unsigned)chunks, 256, smem, s>>>(indices, items, per, (int)experts, chunk_bins);
+    const Plan p = plan_of(items, experts);
+    int32_t *chunk_bins = nullptr, *totals = nullptr;
+    if (p.chunks > 1) {
+        Carver c(workspace);
+        chunk_bins = c.take<int32_t>((size_t)p.chunks * (experts + 1));
+        totals = c.take<int32_t>((size_t)experts + 1);
+        k_plan_count<<<(unsigned)p.chunks, kThreads, (experts + 1) * sizeof(int32_t), s>>>(p, indices, chunk_bins);
+        BGL_LAUNCH_CHECK();
+        k_plan_scan<<<(unsigned)((experts + 8) / 8), kThreads, 0, s>>>(p, chunk_bins, totals, counts);
         BGL_LAUNCH_CHECK();
     }
-    k_plan_scan<<<1, 1024, smem, s>>>(chunk_bins, chunks, (int)experts, counts);
+    k_plan_place<<<(unsigned)(p.chunks > 0 ? p.chunks : 1), p.warps * 32,
+                   p.warps * (experts + 1) * sizeof(int32_t), s>>>(p, indices, chunk_bins, totals,
+                                                                   positions, counts);
     BGL_LAUNCH_CHECK();
-    if (chunks) {
-        k_plan_place<<<(unsigned)chunks, 32, smem, s>>>(indices, items, per, (int)experts,
-                                                        chunk_bins, positions);
-        BGL_LAUNCH_CHECK();
-    }
     return BGL_OK;
 }
 
@@ -225,17 +429,9 @@ int bgl_dispatch_rows(const void *x, const int32_t *positions, int64_t tokens, i
     if (rc) return rc;
     if (tokens == 0 || k == 0 || d == 0) return BGL_OK;
     if (!x || !positions || !rows) return fail(BGL_E_INVALID, "bgl_dispatch_rows: null buffer");
-    cudaStream_t s = as_stream(stream);
-    const unsigned grid = token_blocks(tokens);
-    if (dtype == BGL_F64)
-        k_dispatch<double><<<grid, 256, 0, s>>>((const double *)x, positions, tokens, (int)k, d, (double *)rows);
-    else if (dtype == BGL_F32)
-        k_dispatch<float><<<grid, 256, 0, s>>>((const float *)x, positions, tokens, (int)k, d, (float *)rows);
-    else
-        k_dispatch<__nv_bfloat16><<<grid, 256, 0, s>>>((const __nv_bfloat16 *)x, positions, tokens,
-                                                       (int)k, d, (__nv_bfloat16 *)rows);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    const Rows p = {x, nullptr, positions, nullptr, tokens, d, (int)k, rows, nullptr, as_stream(stream)};
+    if (dtype == BGL_F64) return dispatch_as<double>(p);
+    return dtype == BGL_F32 ? dispatch_as<float>(p) : dispatch_as<__nv_bfloat16>(p);
 }
 
 int bgl_combine_rows(const void *rows, const int32_t *positions, const void *weights,
@@ -244,20 +440,9 @@ int bgl_combine_rows(const void *rows, const int32_t *positions, const void *wei
     if (rc) return rc;
     if (tokens == 0 || d == 0) return BGL_OK;
     if (!y || (k && (!rows || !positions))) return fail(BGL_E_INVALID, "bgl_combine_rows: null buffer");
-    cudaStream_t s = as_stream(stream);
-    const unsigned grid = token_blocks(tokens);
-    if (dtype == BGL_F64)
-        k_combine<double><<<grid, 256, 0, s>>>((const double *)rows, positions, (const double *)weights,
-                                               tokens, (int)k, d, (double *)y);
-    else if (dtype == BGL_F32)
-        k_combine<float><<<grid, 256, 0, s>>>((const float *)rows, positions, (const float *)weights,
-                                              tokens, (int)k, d, (float *)y);
-    else
-        k_combine<__nv_bfloat16><<<grid, 256, 0, s>>>((const __nv_bfloat16 *)rows, positions,
-                                                      (const float *)weights, tokens, (int)k, d,
-                                                      (__nv_bfloat16 *)y);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    const Rows p = {nullptr, rows, positions, weights, tokens, d, (int)k, y, nullptr, as_stream(stream)};
+    if (dtype == BGL_F64) return combine_as<double>(p);
+    return dtype == BGL_F32 ? combine_as<float>(p) : combine_as<__nv_bfloat16>(p);
 }
 
 int bgl_combine_rows_backward(const void *grad, const void *rows, const int32_t *positions,
@@ -268,22 +453,9 @@ int bgl_combine_rows_backward(const void *grad, const void *rows, const int32_t 
     if (tokens == 0 || k == 0) return BGL_OK;
     if (!positions || (d && (!grad || (dweights && !rows))))
         return fail(BGL_E_INVALID, "bgl_combine_rows_backward: null buffer");
-    cudaStream_t s = as_stream(stream);
-    const unsigned grid = token_blocks(tokens);
-    if (dtype == BGL_F64)
-        k_combine_backward<double><<<grid, 256, 0, s>>>(
-            (const double *)grad, (const double *)rows, positions, (const double *)weights, tokens,
-            (int)k, d, (double *)drows, (double *)dweights);
-    else if (dtype == BGL_F32)
-        k_combine_backward<float><<<grid, 256, 0, s>>>(
-            (const float *)grad, (const float *)rows, positions, (const float *)weights, tokens,
-            (int)k, d, (float *)drows, (float *)dweights);
-    else
-        k_combine_backward<__nv_bfloat16><<<grid, 256, 0, s>>>(
-            (const __nv_bfloat16 *)grad, (const __nv_bfloat16 *)rows, positions,
-            (const float *)weights, tokens, (int)k, d, (__nv_bfloat16 *)drows, (float *)dweights);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    const Rows p = {grad, rows, positions, weights, tokens, d, (int)k, drows, dweights, as_stream(stream)};
+    if (dtype == BGL_F64) return combine_backward_as<double>(p);
+    return dtype == BGL_F32 ? combine_backward_as<float>(p) : combine_backward_as<__nv_bfloat16>(p);
 }
 
 }  // extern "C"

@@ -8,6 +8,8 @@ weight and bias may then be float32 or bfloat16.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _tensor as T
@@ -20,10 +22,16 @@ __all__ = ["layer_norm", "layer_norm_backward"]
 def _types(x, *params):
     """Element types of the rows and of the parameters."""
     present = [p for p in params if p is not None]
-    if T.is_bf16(x) and all(T.is_bf16(p) or T.is_f32(p) for p in present):
-        narrow = present and all(T.is_bf16(p) for p in present)
-        return torch.bfloat16, torch.bfloat16 if narrow else torch.float32
-    dtype = T.common_float(*(T.feature(v) for v in (x, *present)))
+    if T.is_bf16(x):
+        narrow = bool(present)
+        for p in present:
+            if not T.is_bf16(p):
+                narrow = False
+                if not T.is_f32(p):
+                    break
+        else:
+            return torch.bfloat16, torch.bfloat16 if narrow else torch.float32
+    dtype = T.float_type(x, *present)
     return dtype, dtype
 
 
@@ -39,10 +47,7 @@ def _check_rows(x, *params):
         if p is not None and T.shape_of(p) != (shape[-1],):
             raise DGLError("{} must have shape ({},), got {}".format(name, shape[-1], T.shape_of(p)))
     d = int(shape[-1])
-    rows = 1
-    for s in shape[:-1]:
-        rows *= int(s)
-    return shape, rows, d
+    return shape, math.prod(shape[:-1]), d
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
@@ -63,11 +68,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     dtype, wdtype = _types(x, weight, bias)
     dev = T.device()
     xt, wt, bt = T.on(dev, x, dtype), T.on(dev, weight, wdtype), T.on(dev, bias, wdtype)
-    y = torch.empty(shape, dtype=dtype, device=dev)
+    y = torch.empty_like(xt)
     mean = rstd = None
     if return_stats:
         mean = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
-        rstd = torch.empty_like(mean)
+        rstd = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
     check(lib().bgl_layer_norm(T.ptr(xt), T.ptr(wt), T.ptr(bt), rows, d, float(eps), T.ptr(y),
                                T.ptr(mean), T.ptr(rstd), T.code_of(dtype), T.code_of(wdtype),
                                T.stream()), "layer_norm")
@@ -95,12 +100,13 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None):
     if T.is_bf16(x) and T.is_bf16(grad):
         dtype, wdtype = _types(x, weight)
     else:
-        dtype = wdtype = T.common_float(*(T.feature(v) for v in (x, grad, weight) if v is not None))
+        present = (x, grad) if weight is None else (x, grad, weight)
+        dtype = wdtype = T.float_type(*present)
     dev = T.device()
     gt, xt = T.on(dev, grad, dtype), T.on(dev, x, dtype)
     mt, rt = T.on(dev, mean, _stat_type(dtype)), T.on(dev, rstd, _stat_type(dtype))
     wt = T.on(dev, weight, wdtype)
-    dx = torch.empty(shape, dtype=dtype, device=dev)
+    dx = torch.empty_like(xt)
     dw = db = ws = None
     nbytes = 0
     if weight is not None:
