@@ -21,7 +21,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBins = 8192;           // experts + 1: shared-memory counters
 constexpr int kCounters = 48 * 1024 / 4; // of a block
-constexpr int kMaxChunks = 2048;
+constexpr int kMaxChunks = 1024;
 
 // ---------------------------------------------------------------- the plan
 // Item i's bin: its expert, or `experts` (the last bin) for none.
@@ -42,10 +42,10 @@ Plan plan_of(int64_t items, int64_t experts) {
     p.experts = (int)experts;
     const int64_t room = kCounters / (experts + 1);
     p.warps = (int)(room < 8 ? room : 8);
-    // 256 items a warp, more where that gave too many chunks; one chunk where 32
+    // 64 items a warp, more where that gave too many chunks; one chunk where 32
     // steps a warp are enough (one launch instead of three)
     int64_t steps = (items + p.warps * 32 * (int64_t)kMaxChunks - 1) / (p.warps * 32 * (int64_t)kMaxChunks);
-    if (steps < 8) steps = 8;
+    if (steps < 2) steps = 2;
     if (items <= p.warps * 32 * 32) steps = (items + p.warps * 32 - 1) / (p.warps * 32);
     p.per_warp = (steps > 0 ? steps : 1) * 32;
     p.chunks = (items + p.per_warp * p.warps - 1) / (p.per_warp * p.warps);
@@ -254,18 +254,20 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // GROUP threads a token, `kFlight` choices at a time: dy is read once for them.
-template <typename T, int GROUP, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+// Warps of a token need no barrier; their blocks are small, so that SMs even out.
+__host__ __device__ constexpr int backward_threads(int group) { return group == 32 ? 128 : group; }
+
+template <typename T, int GROUP, int kFlight, bool VEC>
+__global__ void __launch_bounds__(backward_threads(GROUP))
     k_combine_backward(const T *__restrict__ dy, const T *__restrict__ rows,
                        const int32_t *__restrict__ positions, const Acc<T> *__restrict__ weights,
                        int64_t tokens, int k, int64_t d, T *__restrict__ drows,
                        Acc<T> *__restrict__ dweights) {
     using A = Acc<T>;
     using P = Piece<T, VEC>;
-    constexpr int kFlight = 4;
     __shared__ A smem[32];
     const int own = threadIdx.x % GROUP;
-    const int64_t t = blockIdx.x * (int64_t)(kThreads / GROUP) + threadIdx.x / GROUP;
+    const int64_t t = blockIdx.x * (int64_t)(backward_threads(GROUP) / GROUP) + threadIdx.x / GROUP;
     if (t >= tokens) return;  // whole groups; a group of a block is the block
     for (int j0 = 0; j0 < k; j0 += kFlight) {
         int64_t row[kFlight];
@@ -361,23 +363,26 @@ int combine_as(const Rows &p) {
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }
-template <typename T, int GROUP>
+template <typename T, int GROUP, int FLIGHT>
 int combine_backward_as(const Rows &p) {
     using A = Acc<T>;
     const T *dy = (const T *)p.in, *rows = (const T *)p.rows;
     const A *w = (const A *)p.weights;
-    const unsigned grid = token_blocks(p.tokens, kThreads / GROUP);
+    constexpr int threads = backward_threads(GROUP);
+    const unsigned grid = token_blocks(p.tokens, threads / GROUP);
     if (pieces_of_16<T>(p.d, p.in, p.rows, p.out))
-        k_combine_backward<T, GROUP, true><<<grid, kThreads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
+        k_combine_backward<T, GROUP, FLIGHT, true><<<grid, threads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
     else
-        k_combine_backward<T, GROUP, false><<<grid, kThreads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
+        k_combine_backward<T, GROUP, FLIGHT, false><<<grid, threads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }
 template <typename T>
 int combine_backward_as(const Rows &p) {
-    // a warp a token (no barriers), a block where there are too few tokens for that
-    return p.tokens >= (int64_t)num_sms() * 16 ? combine_backward_as<T, 32>(p) : combine_backward_as<T, kThreads>(p);
+    // a warp a token, a block where there are too few tokens for that
+    if (p.tokens < (int64_t)num_sms() * 16) return combine_backward_as<T, kThreads, 4>(p);
+    // two choices need few registers, and more warps then fit
+    return p.k <= 2 ? combine_backward_as<T, 32, 2>(p) : combine_backward_as<T, 32, 4>(p);
 }
 
 }  // namespace
