@@ -144,6 +144,32 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void 
         : "memory");
 }
 
+// Waits for `slices` whole K slices from number `it` on and multiplies them, 4 MMAs
+// of K = 16 (STEP 16-byte units apart in both operands) for each 128-row half.
+template <int STEP>
+__device__ __forceinline__ bool issue(uint64_t *full, uint64_t *empty, int64_t it, int slices,
+                                      int halves, uint64_t am, uint64_t an, uint32_t idesc,
+                                      uint32_t tmem, volatile int *abort) {
+    int s = (int)(it % kStages);
+    uint32_t parity = (uint32_t)(it / kStages) & 1;
+    for (int k = 0; k < slices; ++k) {
+        if (!mbar_wait(&full[s], parity, 3, abort)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t m = am + s * (kStageBytes / 16), n = an + s * (kStageBytes / 16);
+#pragma unroll
+        for (int kk = 0; kk < kGradSlice / 16; ++kk)
+            mma<true>(tmem, m + kk * STEP, n + kk * STEP, idesc, (k | kk) != 0);
+        if (halves == 2) {
+#pragma unroll
+            for (int kk = 0; kk < kGradSlice / 16; ++kk)
+                mma<true>(tmem + 256u, m + 2 * kBox / 16 + kk * STEP, n + kk * STEP, idesc, (k | kk) != 0);
+        }
+        mma_commit(&empty[s]);
+        if (++s == kStages) s = 0, parity ^= 1;
+    }
+    return true;
+}
+
 // How the roles see an item: the boxes of each operand that are loaded, and the
 // K slices.
 struct Shape {
@@ -270,62 +296,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait(&full[j % kStages], (uint32_t)(j / kStages) & 1, 2, nullptr);
         __syncwarp();
     } else if (warp == kWarpMma) {
+        // One thread issues, in a loop of its own over an item's whole slices: with
+        // the warp taking part in every slice the issue of an MMA took 217 cycles,
+        // where its execution takes 128.
         int64_t it = 0;
         bool ok = true;
         Item q;
         for (int64_t t = 0; ok && take(t, q); ++t) {
             const Shape sh = shape_of(args, q);
-            const uint32_t idesc = q.kind == kDa ? k_instr(sh.n) : mn_instr(sh.n);
-            bool waited = t == 0;  // the epilogue has read the previous tile
-            for (int k = 0; k < sh.slices; ++k, ++it) {
+            const bool da = q.kind == kDa;
+            const uint32_t idesc = da ? k_instr(sh.n) : mn_instr(sh.n);
+            const uint32_t ring_m = smem_u32(ring), ring_n = ring_m + 4 * kBox;
+            const uint64_t am = da ? smem_desc(ring_m) : mn_desc(ring_m);
+            const uint64_t an = da ? smem_desc(ring_n) : mn_desc(ring_n);
+            // slices that are whole; db's last one may not be
+            const int whole = !da && q.rows % kGradSlice ? sh.slices - 1 : sh.slices;
+            if (lane == 0) {
+                for (int h = 0; t > 0 && ok && h < 2; ++h) ok = mbar_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok) ok = da ? issue<2>(full, empty, it, whole, sh.halves, am, an, idesc, tmem, abort)
+                                : issue<128>(full, empty, it, whole, sh.halves, am, an, idesc, tmem, abort);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            it += whole;
+            if (ok && whole < sh.slices) {
                 const int s = (int)(it % kStages);
                 if (!(ok = warp_wait(&full[s], (uint32_t)(it / kStages) & 1, 3, abort))) break;
-                unsigned char *m = ring + s * kStageBytes, *n = m + 4 * kBox;
-                int steps = kGradSlice / 16;
-                if (q.kind == kDb && q.rows - k * kGradSlice < kGradSlice) {
-                    const int rows = q.rows - k * kGradSlice;
-                    steps = (rows + 15) / 16;
-                    const int zero = (steps * 16 - rows) * 8;  // 16-byte pieces of a box
-                    if (zero) {
-                        for (int b = 0; b < 8; ++b) {
-                            if (b < 4 ? b >= sh.boxes_m : b - 4 >= sh.boxes_n) continue;
-                            uint4 *p = reinterpret_cast<uint4 *>(m + b * kBox + rows * 128);
-                            for (int i = lane; i < zero; i += 32) p[i] = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
+                unsigned char *m = ring + s * kStageBytes;
+                const int rows = q.rows % kGradSlice, steps = (rows + 15) / 16;
+                const int zero = (steps * 16 - rows) * 8;  // 16-byte pieces of a box
+                for (int b = 0; b < 8; ++b) {
+                    if (b < 4 ? b >= sh.boxes_m : b - 4 >= sh.boxes_n) continue;
+                    uint4 *p = reinterpret_cast<uint4 *>(m + b * kBox + rows * 128);
+                    for (int i = lane; i < zero; i += 32) p[i] = make_uint4(0, 0, 0, 0);
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int h = 0; h < sh.halves; ++h) {
-                    if (!waited) {
-                        if (!(ok = warp_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    }
-                    if (lane == 0) {
-                        // a half is 128 rows of K runs, or two boxes of 64 columns
-                        const uint32_t am = smem_u32(m + h * 2 * kBox), an = smem_u32(n);
-                        const bool da = q.kind == kDa;
-                        const uint64_t ad = da ? smem_desc(am) : mn_desc(am);
-                        const uint64_t bd = da ? smem_desc(an) : mn_desc(an);
-                        const int step = da ? 2 : 128;  // 16 of K: 32 bytes, or 16 rows of 128
-                        for (int kk = 0; kk < steps; ++kk)
-                            mma<true>(tmem + 256u * h, ad + kk * step, bd + kk * step, idesc,
-                                      (k | kk) != 0);
-                    }
-                    __syncwarp();
-                }
-                if (!ok) break;
-                waited = true;
-                if (lane == 0) mma_commit(&empty[s]);
+                fence_proxy_async_smem();
                 __syncwarp();
+                if (lane == 0) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    for (int h = 0; h < sh.halves; ++h)
+                        for (int kk = 0; kk < steps; ++kk)
+                            mma<true>(tmem + 256u * h, am + (s * kStageBytes + h * 2 * kBox) / 16 + kk * 128,
+                                      an + s * kStageBytes / 16 + kk * 128, idesc, (whole | kk) != 0);
+                    mma_commit(&empty[s]);
+                }
+                ++it;
             }
-            // a half that this tile does not write (both, for a tile without
-            // rows) takes its turn as well: acc_full moves on by one tile only
-            // when every epilogue warp has seen the one before
-            for (int h = waited ? sh.halves : 0; ok && t > 0 && h < 2; ++h)
-                ok = warp_wait(&acc_empty[h], (uint32_t)(t - 1) & 1, 5, abort);
             if (!ok) break;
+            // (all epilogue warps have seen the tile before: they have read it)
             if (lane == 0) mma_commit(acc_full);
             __syncwarp();
         }
