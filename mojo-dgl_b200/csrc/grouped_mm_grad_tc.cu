@@ -170,6 +170,11 @@ __device__ __forceinline__ bool issue(uint64_t *full, uint64_t *empty, int64_t i
     return true;
 }
 
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t lo, uint32_t hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
 // How the roles see an item: the boxes of each operand that are loaded, and the
 // K slices.
 struct Shape {
@@ -359,6 +364,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + 256u * half;
         uint4 *stg = staging + (warp - kWarpEpi0) * 256;
         const int line = half * 128 + quarter * 32;  // first row of the tile here
+        auto release = [&] {  // the accumulators have been read
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[half]);
+        };
         Item q;
         for (int64_t t = 0; take(t, q); ++t) {
             if (!warp_wait(acc_full, (uint32_t)t & 1, 4, abort)) break;
@@ -367,7 +377,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int rows = (da ? q.rows : args.d1 - q.i0) - line;  // those that exist
             const int cols = (da ? args.d1 : args.d2) - q.j0;
             const bool none = !da && q.rows <= 0;
-            for (int c = 0; rows > 0 && c < kGradTile && c < cols; c += 64) {
+            if (q.slot >= 0) {
+                // a piece: float32, [half][16-byte column group][row of the half],
+                // whole lines a warp
+                for (int c = 0; rows > 0 && c < kGradTile && c < cols; c += 64) {
+                    uint32_t v[64];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        tmem_ld16(taddr + (uint32_t)(c + 16 * i),
+                                  *reinterpret_cast<uint32_t(*)[16]>(&v[16 * i]));
+                    tmem_wait_ld();
+                    uint4 *dst = reinterpret_cast<uint4 *>(args.partial + (int64_t)q.slot * kPartial) +
+                                 (half * 64 + c / 4) * 128 + quarter * 32 + lane;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        dst[i * 128] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+                release();
+                continue;
+            }
+            // the tile comes out as bf16 pairs first, so that the accumulators are
+            // free for the next one while this one is stored
+            uint4 o[4][8];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (rows <= 0 || 64 * c >= cols) continue;
                 uint32_t v[64];
                 if (none) {
 #pragma unroll
@@ -375,37 +409,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        tmem_ld16(taddr + (uint32_t)(c + 16 * i),
+                        tmem_ld16(taddr + (uint32_t)(64 * c + 16 * i),
                                   *reinterpret_cast<uint32_t(*)[16]>(&v[16 * i]));
                     tmem_wait_ld();
                 }
-                if (q.slot >= 0) {
-                    // [half][16-byte column group][row of the half]: whole lines a warp
-                    uint4 *dst = reinterpret_cast<uint4 *>(args.partial + (int64_t)q.slot * kPartial) +
-                                 (half * 64 + c / 4) * 128 + quarter * 32 + lane;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        dst[i * 128] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    continue;
-                }
+                for (int j = 0; j < 8; ++j)
+                    o[c][j] = make_uint4(bf16_pair(v[8 * j], v[8 * j + 1]), bf16_pair(v[8 * j + 2], v[8 * j + 3]),
+                                         bf16_pair(v[8 * j + 4], v[8 * j + 5]), bf16_pair(v[8 * j + 6], v[8 * j + 7]));
+            }
+            release();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (rows <= 0 || 64 * c >= cols) continue;
                 if (lane == 0) bulk_wait_read<0>();
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]),
-                                                                  __uint_as_float(v[8 * j + 2 * i + 1]));
-                        o[i] = *reinterpret_cast<uint32_t *>(&h2);
-                    }
-                    stg[lane * 8 + (j ^ (lane & 7))] = make_uint4(o[0], o[1], o[2], o[3]);
-                }
+                for (int j = 0; j < 8; ++j) stg[lane * 8 + (j ^ (lane & 7))] = o[c][j];
                 if (da && rows < 32) {
                     // the segment's last rows: the next segment's must not be written
                     __syncwarp();
                     for (int i = lane; i < rows * 8; i += 32) {
-                        const int row = i >> 3, j = i & 7, col = q.j0 + c + j * 8;
+                        const int row = i >> 3, j = i & 7, col = q.j0 + 64 * c + j * 8;
                         if (col < args.d1)
                             *reinterpret_cast<uint4 *>(args.da + ((int64_t)q.row0 + line + row) * args.d1 + col) =
                                 stg[row * 8 + (j ^ (row & 7))];
@@ -416,16 +441,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) {
                         if (da)
-                            tma_store_2d(&map_da, stg, q.j0 + c, q.row0 + line);
+                            tma_store_2d(&map_da, stg, q.j0 + 64 * c, q.row0 + line);
                         else  // clipped to the segment's block
-                            tma_store_3d(&map_db, stg, q.j0 + c, q.i0 + line, q.seg);
+                            tma_store_3d(&map_db, stg, q.j0 + 64 * c, q.i0 + line, q.seg);
                         bulk_commit();
                     }
                 }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[half]);
         }
         if (lane == 0) bulk_wait_all();
         __syncwarp();
