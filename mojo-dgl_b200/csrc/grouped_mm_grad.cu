@@ -12,29 +12,37 @@ namespace {
 
 constexpr int kTile = 64, kDepth = 16;
 
-// Sum over the block's earlier threads (exclusive), and over all of them.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warps, int64_t &total) {
+// Three sums over the block's earlier threads (exclusive), and over all of them.
+struct Three {
+    int64_t a, b, c;
+};
+__device__ __forceinline__ Three operator+(Three x, Three y) { return {x.a + y.a, x.b + y.b, x.c + y.c}; }
+__device__ __forceinline__ Three operator-(Three x, Three y) { return {x.a - y.a, x.b - y.b, x.c - y.c}; }
+__device__ __forceinline__ Three shfl_up(Three x, int o) {
+    return {__shfl_up_sync(0xffffffffu, x.a, o), __shfl_up_sync(0xffffffffu, x.b, o), __shfl_up_sync(0xffffffffu, x.c, o)};
+}
+__device__ __forceinline__ Three block_scan(Three v, Three *warps, Three &total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockDim.x >> 5;
-    int64_t sum = v;
+    Three sum = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
+        const Three up = shfl_up(sum, o);
+        if (lane >= o) sum = sum + up;
     }
     if (lane == 31) warps[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-        int64_t w = lane < n ? warps[lane] : 0;
+        Three w = lane < n ? warps[lane] : Three{0, 0, 0};
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += up;
+            const Three up = shfl_up(w, o);
+            if (lane >= o) w = w + up;
         }
         warps[lane] = w;
     }
     __syncthreads();
     total = warps[n - 1];
-    const int64_t before = (warp ? warps[warp - 1] : 0) + sum - v;
+    const Three before = (warp ? warps[warp - 1] : Three{0, 0, 0}) + sum - v;
     __syncthreads();
     return before;
 }
@@ -55,34 +63,47 @@ __global__ void __launch_bounds__(1024)
                     int64_t slices2, bool want_da, bool want_db, GradLayout l) {
     constexpr int64_t kTileCost = 4, kShortest = 8;
     constexpr int kSorted = 256;  // more segments than this stay in order
-    __shared__ int64_t warps[32];
+    __shared__ Three warps[32];
     __shared__ int64_t lens[kSorted];
     int64_t rows = 0, tiles = 0, slices = 0;
     for (int64_t i0 = 0; i0 < r; i0 += blockDim.x) {
         const int64_t i = i0 + threadIdx.x;
-        int64_t len = i < r ? seglen[i] : 0, total;
+        int64_t len = i < r ? seglen[i] : 0;
         len = len < 0 ? 0 : len < n ? len : n;
-        const int64_t row = rows + block_scan(len, warps, total);
-        const int64_t first = row < n ? row : n, end = row + len < n ? row + len : n;
-        rows += total;
-        const int64_t tile = tiles + block_scan((end - first + kGradTile - 1) / kGradTile, warps, total);
-        tiles += total;
+        // (the tiles are those of the rows that there are: where lengths add up
+        // to more than n, which no caller of a matching product gives, a second
+        // scan counts them)
+        Three total;
+        Three before = block_scan({len, (len + kGradTile - 1) / kGradTile, 0}, warps, total);
+        int64_t first = rows + before.a, end = first + len;
+        if (rows + total.a > n) {
+            first = first < n ? first : n;
+            end = end < n ? end : n;
+            Three clamped;
+            before.b = block_scan({0, (end - first + kGradTile - 1) / kGradTile, 0}, warps, clamped).b;
+            total.b = clamped.b;
+        }
         int64_t mine = (end - first + kGradSlice - 1) / kGradSlice;
         if (i < r && mine == 0) mine = 1;  // a segment without rows: one piece a tile writes zeros
-        block_scan(mine, warps, total);
-        slices += total;
         if (i < r) {
             l.off[i] = first;
-            l.row_off[i] = tile;
+            l.row_off[i] = tiles + before.b;
             if (r <= kSorted) lens[i] = mine;
         }
+        slices += mine;
+        rows += total.a;
+        tiles += total.b;
     }
     if (threadIdx.x == 0) {
         l.off[r] = rows < n ? rows : n;
         l.row_off[r] = tiles;
     }
-    __syncthreads();
     if (!want_da && !want_db) return;
+    {
+        Three total;
+        block_scan({slices, 0, 0}, warps, total);
+        slices = total.a;
+    }
     for (int64_t i = threadIdx.x; i < r; i += blockDim.x) {
         int64_t at = i;
         if (r <= kSorted) {
@@ -101,23 +122,24 @@ __global__ void __launch_bounds__(1024)
     int64_t items = 0, cut = 0, slots = 0;
     for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {
         const int64_t k = k0 + threadIdx.x;
-        int64_t pieces = 0, total;
+        int64_t pieces = 0;
         if (k < r) {
             const int32_t seg = l.order[k];
             const int64_t len = l.off[seg + 1] - l.off[seg];
             pieces = grad_pieces(len, piece).count;
         }
-        const int64_t item = items + block_scan(pieces * per_segment, warps, total);
-        items += total;
-        const int64_t c = cut + block_scan(pieces > 1 ? per_segment : 0, warps, total);
-        cut += total;
-        const int64_t slot = slots + block_scan(pieces > 1 ? pieces * per_segment : 0, warps, total);
-        slots += total;
+        const bool several = pieces > 1;
+        Three total;
+        const Three before = block_scan({pieces * per_segment, several ? per_segment : 0,
+                                         several ? pieces * per_segment : 0}, warps, total);
         if (k < r) {
-            l.item_off[k] = item;
-            l.cut_off[k] = c;
-            l.slot_off[k] = slot;
+            l.item_off[k] = items + before.a;
+            l.cut_off[k] = cut + before.b;
+            l.slot_off[k] = slots + before.c;
         }
+        items += total.a;
+        cut += total.b;
+        slots += total.c;
     }
     if (threadIdx.x == 0) {
         l.item_off[r] = items;
@@ -319,7 +341,8 @@ int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, cons
     const GradTiles t = gmm_grad_tiles(n, d1, r, d2);
     const bool tc = r && gmm_grad_tc_supported(grad, a, b, want_da ? da : nullptr,
                                                want_db ? db : nullptr, n, d1, r, d2, dtype);
-    k_grad_schedule<<<1, 1024, 0, s>>>(seglen, r, n, t, (d2 + kGradSlice - 1) / kGradSlice,
+    const unsigned threads = r < 1024 ? (unsigned)(r + 31) / 32 * 32 : 1024;
+    k_grad_schedule<<<1, threads ? threads : 32, 0, s>>>(seglen, r, n, t, (d2 + kGradSlice - 1) / kGradSlice,
                                        tc && want_da, tc && want_db, l);
     BGL_LAUNCH_CHECK();
     if (!want_da) da = nullptr;

@@ -149,9 +149,21 @@ def to_dev(a, dtype: torch.dtype = None) -> torch.Tensor:
     return t.to(dev)
 
 
-def array(a):
-    """The operand with a shape and an element type: lists become numpy arrays."""
-    return a if a is None or is_torch(a) else np.asanyarray(a)
+def operands(*xs):
+    """``kind_of`` the operands, and the operands with a shape and an element
+    type each: lists become numpy arrays, an absent one stays None."""
+    kind, plain = NUMPY, False
+    for x in xs:
+        if isinstance(x, torch.Tensor):
+            if x.is_cuda:
+                kind = TORCH_CUDA
+            elif kind == NUMPY:
+                kind = TORCH_CPU
+        elif x is not None:
+            plain = True
+    if plain:
+        xs = tuple(x if x is None or isinstance(x, torch.Tensor) else np.asanyarray(x) for x in xs)
+    return kind, xs
 
 
 def is_bf16(a) -> bool:
@@ -183,6 +195,11 @@ def on(dev: torch.device, a, dtype: torch.dtype):
     if isinstance(a, torch.Tensor) and a.dtype is dtype and a.device == dev and a.is_contiguous():
         return a
     return to_dev(a, dtype)
+
+
+def address(t) -> int:
+    """Device address of a tensor, None (NULL) for an absent one."""
+    return None if t is None else t.data_ptr()
 
 
 def result(t: torch.Tensor, kind: int):

@@ -10,7 +10,8 @@ A mixture-of-experts layer on this package's grouped products::
 
 ``segment_mm_backward``, ``combine_backward`` and ``route_topk_backward`` lead
 back; the gradient of ``dispatch`` is ``combine`` without weights.  None of the
-functions here reads device data on the host.
+functions here waits for the device (indices given as floats excepted, which are
+checked to be whole numbers).
 """
 
 from __future__ import annotations
@@ -31,7 +32,7 @@ __all__ = ["route_topk", "route_topk_backward", "ExpertPlan", "expert_plan", "di
 # -------------------------------------------------------------------- routing
 def _logits(logits):
     """The logits as float32 or bfloat16, with their element type."""
-    if len(T.shape_of(logits)) != 2:
+    if logits.ndim != 2:
         raise DGLError("logits must be (tokens, experts), got shape {}".format(T.shape_of(logits)))
     if T.is_bf16(logits):
         return torch.bfloat16
@@ -69,10 +70,9 @@ def route_topk(logits, k, *, score="softmax", bias=None, num_groups=1, topk_grou
     left (a padding token has none) gets index -1 and weight 0 in the remaining
     places.  Returns (weights, indices), float32 and int64, both (tokens, k).
     """
-    kind = T.kind_of(logits, bias)
-    logits, bias = T.array(logits), T.array(bias)
+    kind, (logits, bias) = T.operands(logits, bias)
     dtype = _logits(logits)
-    tokens, experts = (int(v) for v in T.shape_of(logits))
+    tokens, experts = logits.shape
     k, code = _choices(k, experts), _score(score)
     num_groups = int(num_groups)
     topk_groups = num_groups if topk_groups is None else int(topk_groups)
@@ -91,9 +91,9 @@ def route_topk(logits, k, *, score="softmax", bias=None, num_groups=1, topk_grou
     lt, bt = T.on(dev, logits, dtype), T.on(dev, bias, torch.float32)
     weights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
     indices = torch.empty((tokens, k), dtype=torch.int64, device=dev)
-    check(lib().bgl_route_topk(T.ptr(lt), T.ptr(bt), tokens, experts, k, code, num_groups,
+    check(lib().bgl_route_topk(T.address(lt), T.address(bt), tokens, experts, k, code, num_groups,
                                topk_groups, group_top, int(bool(renormalize)), float(scale),
-                               T.ptr(weights), T.ptr(indices), T.code_of(dtype), T.stream()),
+                               T.address(weights), T.address(indices), T.code_of(dtype), T.stream()),
           "route_topk")
     return T.result(weights, kind), T.result(indices, kind)
 
@@ -107,22 +107,22 @@ def route_topk_backward(grad, logits, indices, *, score="softmax", renormalize=T
     that is not an expert's) have none either.  Returns (tokens, experts) in the
     logits' type.
     """
-    kind = T.kind_of(grad, logits, indices)
-    grad, logits, indices = T.array(grad), T.array(logits), T.array(indices)
+    kind, (grad, logits, indices) = T.operands(grad, logits, indices)
     dtype = _logits(logits)
-    tokens, experts = (int(v) for v in T.shape_of(logits))
+    tokens, experts = logits.shape
     shape = T.shape_of(indices)
     if len(shape) != 2 or shape[0] != tokens:
         raise DGLError("indices must be ({}, k), got shape {}".format(tokens, shape))
     k, code = _choices(shape[1], experts), _score(score)
     if T.shape_of(grad) != shape:
         raise DGLError("grad must have the shape of indices, {}, got {}".format(shape, T.shape_of(grad)))
+    indices = T.ids(indices)
     dev = T.device()
     gt, lt = T.on(dev, grad, torch.float32), T.on(dev, logits, dtype)
-    it = T.on(dev, T.ids(indices), torch.int64)
-    dlogits = torch.empty((tokens, experts), dtype=dtype, device=dev)
-    check(lib().bgl_route_topk_backward(T.ptr(gt), T.ptr(lt), T.ptr(it), tokens, experts, k, code,
-                                        int(bool(renormalize)), float(scale), T.ptr(dlogits),
+    it = T.on(dev, indices, torch.int64)
+    dlogits = torch.empty_like(lt)
+    check(lib().bgl_route_topk_backward(T.address(gt), T.address(lt), T.address(it), tokens, experts, k, code,
+                                        int(bool(renormalize)), float(scale), T.address(dlogits),
                                         T.code_of(dtype), T.stream()), "route_topk_backward")
     return T.result(dlogits, kind)
 
@@ -144,29 +144,31 @@ def expert_plan(indices, num_experts):
     ``indices`` is (tokens, k); an index outside [0, ``num_experts``), such as
     the -1 of a padding token, goes to no expert.
     """
-    kind = T.kind_of(indices)
-    indices = T.array(indices)
+    kind, (indices,) = T.operands(indices)
     if len(T.shape_of(indices)) != 2:
         raise DGLError("indices must be (tokens, k), got shape {}".format(T.shape_of(indices)))
     experts = int(num_experts)
     if experts < 1:
         raise DGLError("num_experts must be positive, got {}".format(experts))
+    indices = T.ids(indices)
     dev = T.device()
-    it = T.on(dev, T.ids(indices), torch.int64)
+    it = T.on(dev, indices, torch.int64)
     items = it.numel()
     counts = torch.empty(experts, dtype=torch.int64, device=dev)
     positions = torch.empty(it.shape, dtype=torch.int32, device=dev)
     nbytes = lib().bgl_expert_plan_workspace_size(items, experts)
-    ws = T.workspace(nbytes)
-    check(lib().bgl_expert_plan(T.ptr(it), items, experts, T.ptr(counts), T.ptr(positions),
-                                T.ptr(ws), nbytes, T.stream()), "expert_plan")
+    ws = T.workspace(nbytes) if nbytes else None
+    check(lib().bgl_expert_plan(T.address(it), items, experts, T.address(counts), T.address(positions),
+                                T.address(ws), nbytes, T.stream()), "expert_plan")
     return ExpertPlan(T.result(counts, kind), T.result(positions, kind))
 
 
 def _positions(positions):
-    shape = T.shape_of(positions)
+    shape = positions.shape
     if len(shape) != 2:
-        raise DGLError("positions must be (tokens, k), got shape {}".format(shape))
+        raise DGLError("positions must be (tokens, k), got shape {}".format(tuple(shape)))
+    if positions.dtype is torch.int32:
+        return shape
     if T.is_torch(positions):
         whole = not (positions.is_floating_point() or positions.is_complex()
                      or positions.dtype == torch.bool)
@@ -174,19 +176,18 @@ def _positions(positions):
         whole = np.issubdtype(positions.dtype, np.integer)
     if not whole:
         raise DGLError("positions must be whole numbers, got {}".format(positions.dtype))
-    return int(shape[0]), int(shape[1])
+    return shape
 
 
-def _matrix(x, what, rows=None):
-    shape = T.shape_of(x)
-    if len(shape) != 2 or (rows is not None and shape[0] != rows):
-        raise DGLError("{} must be ({}, D), got shape {}".format(
-            what, "rows" if rows is None else rows, shape))
-    return int(shape[1])
+def _matrix(x, what, rows):
+    shape = x.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise DGLError("{} must be ({}, D), got shape {}".format(what, rows, tuple(shape)))
+    return shape[1]
 
 
 def _weights(weights, tokens, k):
-    if weights is not None and T.shape_of(weights) != (tokens, k):
+    if weights is not None and tuple(weights.shape) != (tokens, k):
         raise DGLError("weights must be ({}, {}), got shape {}".format(tokens, k, T.shape_of(weights)))
 
 
@@ -201,15 +202,14 @@ def dispatch(x, positions):
     of choices without an expert, behind all others, are zeros.  The gradient
     with respect to x is ``combine(grad, positions)``.
     """
-    kind = T.kind_of(x, positions)
-    x, positions = T.array(x), T.array(positions)
+    kind, (x, positions) = T.operands(x, positions)
     tokens, k = _positions(positions)
     d = _matrix(x, "x", tokens)
     dtype = T.float_type(x)
     dev = T.device()
     xt, pt = T.on(dev, x, dtype), T.on(dev, positions, torch.int32)
-    rows = torch.empty((tokens * k, d), dtype=dtype, device=dev)
-    check(lib().bgl_dispatch_rows(T.ptr(xt), T.ptr(pt), tokens, k, d, T.ptr(rows),
+    rows = xt.new_empty((tokens * k, d))
+    check(lib().bgl_dispatch_rows(T.address(xt), T.address(pt), tokens, k, d, T.address(rows),
                                   T.code_of(dtype), T.stream()), "dispatch")
     return T.result(rows, kind)
 
@@ -222,8 +222,7 @@ def combine(rows, positions, weights=None):
     choices without an expert add nothing, whatever their weight.  Sums run in
     float32 (float64 for float64 rows) in the order of the choices.
     """
-    kind = T.kind_of(rows, positions, weights)
-    rows, positions, weights = T.array(rows), T.array(positions), T.array(weights)
+    kind, (rows, positions, weights) = T.operands(rows, positions, weights)
     tokens, k = _positions(positions)
     d = _matrix(rows, "rows", tokens * k)
     _weights(weights, tokens, k)
@@ -231,8 +230,8 @@ def combine(rows, positions, weights=None):
     dev = T.device()
     rt, pt = T.on(dev, rows, dtype), T.on(dev, positions, torch.int32)
     wt = T.on(dev, weights, _weight_type(dtype))
-    y = torch.empty((tokens, d), dtype=dtype, device=dev)
-    check(lib().bgl_combine_rows(T.ptr(rt), T.ptr(pt), T.ptr(wt), tokens, k, d, T.ptr(y),
+    y = rt.new_empty((tokens, d))
+    check(lib().bgl_combine_rows(T.address(rt), T.address(pt), T.address(wt), tokens, k, d, T.address(y),
                                  T.code_of(dtype), T.stream()), "combine")
     return T.result(y, kind)
 
@@ -245,9 +244,7 @@ def combine_backward(grad, rows, positions, weights=None):
     Choices without an expert get rows of zeros and a weight gradient of 0.
     Returns (drows, dweights), the latter None without weights.
     """
-    kind = T.kind_of(grad, rows, positions, weights)
-    grad, rows, positions = T.array(grad), T.array(rows), T.array(positions)
-    weights = T.array(weights)
+    kind, (grad, rows, positions, weights) = T.operands(grad, rows, positions, weights)
     tokens, k = _positions(positions)
     d = _matrix(rows, "rows", tokens * k)
     if T.shape_of(grad) != (tokens, d):
@@ -257,11 +254,11 @@ def combine_backward(grad, rows, positions, weights=None):
     dev = T.device()
     gt, rt, pt = T.on(dev, grad, dtype), T.on(dev, rows, dtype), T.on(dev, positions, torch.int32)
     wt = T.on(dev, weights, _weight_type(dtype))
-    drows = torch.empty((tokens * k, d), dtype=dtype, device=dev)
+    drows = torch.empty_like(rt)
     dweights = None
     if weights is not None:
-        dweights = torch.empty((tokens, k), dtype=_weight_type(dtype), device=dev)
-    check(lib().bgl_combine_rows_backward(T.ptr(gt), T.ptr(rt), T.ptr(pt), T.ptr(wt), tokens, k, d,
-                                          T.ptr(drows), T.ptr(dweights), T.code_of(dtype),
+        dweights = torch.empty_like(wt)
+    check(lib().bgl_combine_rows_backward(T.address(gt), T.address(rt), T.address(pt), T.address(wt), tokens, k, d,
+                                          T.address(drows), T.address(dweights), T.code_of(dtype),
                                           T.stream()), "combine_backward")
     return T.result(drows, kind), None if weights is None else T.result(dweights, kind)

@@ -39,14 +39,14 @@ def _stat_type(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
-def _check_rows(x, *params):
-    shape = T.shape_of(x)
+def _check_rows(x, weight, bias):
+    shape = tuple(x.shape)
     if not shape or shape[-1] < 1:
         raise DGLError("layer norm needs a last axis of at least one value, got shape {}".format(shape))
-    for name, p in params:
-        if p is not None and T.shape_of(p) != (shape[-1],):
-            raise DGLError("{} must have shape ({},), got {}".format(name, shape[-1], T.shape_of(p)))
-    d = int(shape[-1])
+    d = shape[-1]
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.ndim != 1 or p.shape[0] != d):
+            raise DGLError("{} must have shape ({},), got {}".format(name, d, tuple(p.shape)))
     return shape, math.prod(shape[:-1]), d
 
 
@@ -62,9 +62,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
         raise DGLError("layer_norm takes a bias only together with a weight")
     if not eps >= 0:
         raise DGLError("eps must not be negative, got {}".format(eps))
-    kind = T.kind_of(x, weight, bias)
-    x, weight, bias = T.array(x), T.array(weight), T.array(bias)
-    shape, rows, d = _check_rows(x, ("weight", weight), ("bias", bias))
+    kind, (x, weight, bias) = T.operands(x, weight, bias)
+    shape, rows, d = _check_rows(x, weight, bias)
     dtype, wdtype = _types(x, weight, bias)
     dev = T.device()
     xt, wt, bt = T.on(dev, x, dtype), T.on(dev, weight, wdtype), T.on(dev, bias, wdtype)
@@ -73,8 +72,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     if return_stats:
         mean = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
         rstd = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
-    check(lib().bgl_layer_norm(T.ptr(xt), T.ptr(wt), T.ptr(bt), rows, d, float(eps), T.ptr(y),
-                               T.ptr(mean), T.ptr(rstd), T.code_of(dtype), T.code_of(wdtype),
+    check(lib().bgl_layer_norm(T.address(xt), T.address(wt), T.address(bt), rows, d, float(eps), T.address(y),
+                               T.address(mean), T.address(rstd), T.code_of(dtype), T.code_of(wdtype),
                                T.stream()), "layer_norm")
     if not return_stats:
         return T.result(y, kind)
@@ -89,9 +88,8 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None):
     weight.  The sums over rows have a fixed order: the same inputs give the
     same bits.
     """
-    kind = T.kind_of(grad, x, mean, rstd, weight)
-    grad, x, mean, rstd, weight = (T.array(v) for v in (grad, x, mean, rstd, weight))
-    shape, rows, d = _check_rows(x, ("weight", weight))
+    kind, (grad, x, mean, rstd, weight) = T.operands(grad, x, mean, rstd, weight)
+    shape, rows, d = _check_rows(x, weight, None)
     if T.shape_of(grad) != shape:
         raise DGLError("grad must have the shape of x, {}, got {}".format(shape, T.shape_of(grad)))
     for name, s in (("mean", mean), ("rstd", rstd)):
@@ -113,9 +111,9 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None):
         dw, db = torch.empty((2, d), dtype=wdtype, device=dev).unbind(0)
         nbytes = lib().bgl_layer_norm_backward_workspace_size(rows, d, T.code_of(dtype))
         ws = T.workspace(nbytes)
-    check(lib().bgl_layer_norm_backward(T.ptr(gt), T.ptr(xt), T.ptr(mt), T.ptr(rt), T.ptr(wt), rows,
-                                        d, T.ptr(dx), T.ptr(dw), T.ptr(db), T.code_of(dtype),
-                                        T.code_of(wdtype), T.ptr(ws), nbytes, T.stream()),
+    check(lib().bgl_layer_norm_backward(T.address(gt), T.address(xt), T.address(mt), T.address(rt), T.address(wt), rows,
+                                        d, T.address(dx), T.address(dw), T.address(db), T.code_of(dtype),
+                                        T.code_of(wdtype), T.address(ws), nbytes, T.stream()),
           "layer_norm_backward")
     if weight is None:
         return T.result(dx, kind), None, None

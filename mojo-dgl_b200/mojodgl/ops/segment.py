@@ -157,12 +157,11 @@ def segment_mm_backward(grad, a, b, seglen_a, need_a=True, need_b=True):
     N.  bfloat16 tensors run in BF16 with float32 sums, float32 and float64
     exactly.
     """
-    kind = T.kind_of(grad, a, b, seglen_a)
-    grad, a, b = T.array(grad), T.array(a), T.array(b)
-    if len(T.shape_of(a)) != 2 or len(T.shape_of(b)) != 3:
+    kind, (grad, a, b, seglen_a) = T.operands(grad, a, b, seglen_a)
+    if a.ndim != 2 or b.ndim != 3:
         raise DGLError("segment_mm_backward wants a 2-D left operand and a 3-D right operand")
-    n, d1 = (int(v) for v in T.shape_of(a))
-    r, b_d1, d2 = (int(v) for v in T.shape_of(b))
+    n, d1 = a.shape
+    r, b_d1, d2 = b.shape
     if b_d1 != d1:
         raise DGLError("inner dimensions do not match: {} vs {}".format(d1, b_d1))
     if T.shape_of(grad) != (n, d2):
@@ -177,12 +176,12 @@ def segment_mm_backward(grad, a, b, seglen_a, need_a=True, need_b=True):
     dev = T.device()
     gt, at, bt = T.on(dev, grad, dtype), T.on(dev, a, dtype), T.on(dev, b, dtype)
     st = T.on(dev, seg, torch.int64)
-    da = torch.empty((n, d1), dtype=dtype, device=dev) if need_a else None
-    db = torch.empty((r, d1, d2), dtype=dtype, device=dev) if need_b else None
+    da = torch.empty_like(at) if need_a else None
+    db = torch.empty_like(bt) if need_b else None
     code = T.code_of(dtype)
     nbytes = lib().bgl_segment_mm_backward_workspace_size(n, d1, r, d2, code)
     ws = T.workspace(nbytes)
-    check(lib().bgl_segment_mm_backward(T.ptr(gt), T.ptr(at), T.ptr(bt), T.ptr(st), n, d1, r, d2,
-                                        T.ptr(da), T.ptr(db), code, T.ptr(ws), nbytes, T.stream()),
+    check(lib().bgl_segment_mm_backward(T.address(gt), T.address(at), T.address(bt), T.address(st), n, d1, r, d2,
+                                        T.address(da), T.address(db), code, T.address(ws), nbytes, T.stream()),
           "segment_mm_backward")
     return T.result(da, kind) if need_a else None, T.result(db, kind) if need_b else None
