@@ -53,15 +53,16 @@ __device__ __forceinline__ Three block_scan(Three v, Three *warps, Three &total)
 //
 // Items are taken by whichever CTA is free, db's first and its long segments
 // first, da's small tiles last, so the CTAs end together.  A db tile is cut
-// into pieces only where its sum would outlast the rest: its pieces have at
-// most (da's work + half of db's) / CTAs slices, which also bounds the partial
-// tiles (a sum of L slices cut into pieces of P has ceil(L / P) < 2 L / P of
-// them where L > P, all sums together 2 * work / P <= 4 a CTA).  A tile's
-// read-out counts as kTileCost slices (2.4 us against 0.55 us a slice).
+// into pieces where its sum is longer than half of a CTA's share of all work;
+// that also bounds the partial tiles (a sum of L slices cut into pieces of P has
+// ceil(L / P) < 2 L / P of them where L > P, all sums together 2 * work / P <= 4 a
+// CTA).  A tile's read-out counts as kTileCost slices.  Measured with 500000 x 256
+// x 256 over 64 segments (7,860 slices of db, 2,017 tiles of da): 240 us where
+// pieces could be as long as a CTA's share, 226 us so.
 __global__ void __launch_bounds__(1024)
     k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, GradTiles t,
                     int64_t slices2, bool want_da, bool want_db, GradLayout l) {
-    constexpr int64_t kTileCost = 4, kShortest = 8;
+    constexpr int64_t kTileCost = 2, kShortest = 8;
     constexpr int kSorted = 256;  // more segments than this stay in order
     __shared__ Three warps[32];
     __shared__ int64_t lens[kSorted];
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(1024)
     const int64_t da_items = want_da ? tiles * t.tiles1 : 0;
     const int64_t da_work = da_items * (slices2 + kTileCost);
     const int64_t db_work = slices * per_segment;
-    int64_t piece = (da_work + db_work / 2 + t.ctas - 1) / t.ctas;
+    int64_t piece = (da_work + db_work + 2 * t.ctas - 1) / (2 * t.ctas);
     if (piece < kShortest) piece = kShortest;
     int64_t items = 0, cut = 0, slots = 0;
     for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {

@@ -488,16 +488,25 @@ __global__ void __launch_bounds__(256) k_grad_finish(const GradArgs args) {
                             (half * 64 + group * 4) * 128 + line;
         float4 sum[4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum[v] = src[v * 128];
-        for (int64_t p = 1; p < count; ++p) {
+        for (int v = 0; v < 4; ++v) sum[v] = make_float4(0, 0, 0, 0);
+        constexpr int kFlight = 4;  // pieces under way
+        for (int64_t p0 = 0; p0 < count; p0 += kFlight) {
+            float4 x[kFlight][4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float4 x = src[p * (kPartial / 4) + v * 128];
-                sum[v].x += x.x;
-                sum[v].y += x.y;
-                sum[v].z += x.z;
-                sum[v].w += x.w;
-            }
+            for (int p = 0; p < kFlight; ++p)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    x[p][v] = p0 + p < count ? __ldcs(src + (p0 + p) * (kPartial / 4) + v * 128)
+                                             : make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int p = 0; p < kFlight; ++p)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    sum[v].x += x[p][v].x;
+                    sum[v].y += x[p][v].y;
+                    sum[v].z += x[p][v].z;
+                    sum[v].w += x[p][v].w;
+                }
         }
         __nv_bfloat16 *dst = args.db + (seg * (int64_t)args.d1 + i) * args.d2 + j;
 #pragma unroll
