@@ -89,8 +89,8 @@ def route_topk(logits, k, *, score="softmax", bias=None, num_groups=1, topk_grou
         raise DGLError("bias must have shape ({},), got {}".format(experts, T.shape_of(bias)))
     dev = T.device()
     lt, bt = T.on(dev, logits, dtype), T.on(dev, bias, torch.float32)
-    weights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
-    indices = torch.empty((tokens, k), dtype=torch.int64, device=dev)
+    weights = torch.empty(tokens, k, dtype=torch.float32, device=dev)
+    indices = torch.empty_like(weights, dtype=torch.int64)
     check(lib().bgl_route_topk(T.address(lt), T.address(bt), tokens, experts, k, code, num_groups,
                                topk_groups, group_top, int(bool(renormalize)), float(scale),
                                T.address(weights), T.address(indices), T.code_of(dtype), T.stream()),
@@ -155,7 +155,7 @@ def expert_plan(indices, num_experts):
     it = T.on(dev, indices, torch.int64)
     items = it.numel()
     counts = torch.empty(experts, dtype=torch.int64, device=dev)
-    positions = torch.empty(it.shape, dtype=torch.int32, device=dev)
+    positions = torch.empty_like(it, dtype=torch.int32)
     nbytes = lib().bgl_expert_plan_workspace_size(items, experts)
     ws = T.workspace(nbytes) if nbytes else None
     check(lib().bgl_expert_plan(T.address(it), items, experts, T.address(counts), T.address(positions),
@@ -208,7 +208,7 @@ def dispatch(x, positions):
     dtype = T.float_type(x)
     dev = T.device()
     xt, pt = T.on(dev, x, dtype), T.on(dev, positions, torch.int32)
-    rows = xt.new_empty((tokens * k, d))
+    rows = xt.new_empty(tokens * k, d)
     check(lib().bgl_dispatch_rows(T.address(xt), T.address(pt), tokens, k, d, T.address(rows),
                                   T.code_of(dtype), T.stream()), "dispatch")
     return T.result(rows, kind)
@@ -230,7 +230,7 @@ def combine(rows, positions, weights=None):
     dev = T.device()
     rt, pt = T.on(dev, rows, dtype), T.on(dev, positions, torch.int32)
     wt = T.on(dev, weights, _weight_type(dtype))
-    y = rt.new_empty((tokens, d))
+    y = rt.new_empty(tokens, d)
     check(lib().bgl_combine_rows(T.address(rt), T.address(pt), T.address(wt), tokens, k, d, T.address(y),
                                  T.code_of(dtype), T.stream()), "combine")
     return T.result(y, kind)

@@ -70,8 +70,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
     y = torch.empty_like(xt)
     mean = rstd = None
     if return_stats:
-        mean = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
-        rstd = torch.empty(shape[:-1], dtype=_stat_type(dtype), device=dev)
+        lead = shape[:-1]  # (sizes one by one: torch parses them faster than a tuple)
+        mean = torch.empty(*lead or ((),), dtype=_stat_type(dtype), device=dev)
+        rstd = torch.empty_like(mean)
     check(lib().bgl_layer_norm(T.address(xt), T.address(wt), T.address(bt), rows, d, float(eps), T.address(y),
                                T.address(mean), T.address(rstd), T.code_of(dtype), T.code_of(wdtype),
                                T.stream()), "layer_norm")
@@ -108,7 +109,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None):
     dw = db = ws = None
     nbytes = 0
     if weight is not None:
-        dw, db = torch.empty((2, d), dtype=wdtype, device=dev).unbind(0)
+        dw, db = torch.empty_like(wt), torch.empty_like(wt)
         nbytes = lib().bgl_layer_norm_backward_workspace_size(rows, d, T.code_of(dtype))
         ws = T.workspace(nbytes)
     check(lib().bgl_layer_norm_backward(T.address(gt), T.address(xt), T.address(mt), T.address(rt), T.address(wt), rows,
