@@ -108,25 +108,21 @@ __device__ __forceinline__ void Piece<__nv_bfloat16, true>::set(int i, Pair<floa
     *reinterpret_cast<__nv_bfloat162 *>(&v[2 * i]) = __floats2bfloat162_rn(p.x, p.y);
 }
 
-// The parameters of a piece at p, in 16-byte loads where VEC.
-template <typename T, bool VEC, typename W>
-__device__ __forceinline__ void load_params(const W *p, int64_t left, Pair<Acc<T>> (&v)[Piece<T, VEC>::kPairs]) {
+// The parameters of a 16-byte piece at p, 16-byte aligned.
+template <typename T, typename W>
+__device__ __forceinline__ void load_params(const W *p, Pair<Acc<T>> (&v)[Piece<T, true>::kPairs]) {
     using A = Acc<T>;
-    if constexpr (VEC) {
-        constexpr int kWide = 16 / (int)sizeof(W), kLoads = Piece<T, true>::kWide / kWide;
+    constexpr int kWide = 16 / (int)sizeof(W), kLoads = Piece<T, true>::kWide / kWide;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            union {
-                uint4 raw;
-                W w[kWide];
-            } u;
-            u.raw = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    for (int i = 0; i < kLoads; ++i) {
+        union {
+            uint4 raw;
+            W w[kWide];
+        } u;
+        u.raw = __ldg(reinterpret_cast<const uint4 *>(p) + i);
 #pragma unroll
-            for (int j = 0; j < kWide / 2; ++j)
-                v[i * (kWide / 2) + j] = {A(to_acc(u.w[2 * j])), A(to_acc(u.w[2 * j + 1]))};
-        }
-    } else {
-        v[0] = {A(to_acc(p[0])), left > 1 ? A(to_acc(p[1])) : A(0)};
+        for (int j = 0; j < kWide / 2; ++j)
+            v[i * (kWide / 2) + j] = {A(to_acc(u.w[2 * j])), A(to_acc(u.w[2 * j + 1]))};
     }
 }
 
@@ -164,42 +160,126 @@ __host__ __device__ constexpr int forward_resident(int group, int values, int si
     return (size == 8 ? 3 : values == 8 ? 5 : 4) * kThreads / threads_of(group);
 }
 
-template <typename T, typename W, int GROUP, int N, bool VEC>
+// A thread's columns in the rows of its group: piece i holds the values from
+// column(i) on.  kShifted: the pieces are the aligned ones inside the row; what is
+// before and behind them goes to the group's first threads, one value each (the
+// thread's `extra` column).
+template <typename T, int GROUP, int MODE>
+struct Columns {
+    using P = Piece<T, MODE != kScalar>;
+    int t, head, end;  // first column of the pieces, and the one behind them
+    int extra;         // -1: none
+
+    __device__ __forceinline__ Columns(int64_t first_row, int64_t d) : t(threadIdx.x % GROUP), head(0), end((int)d), extra(-1) {
+        if (MODE == kShifted) {
+            head = (int)(-(uint64_t)(first_row * d) % P::kWide);
+            if (head > d) head = (int)d;
+            end = head + ((int)d - head) / P::kWide * P::kWide;
+            if (t < head) extra = t;
+            else if (t < head + (int)d - end) extra = end + t - head;
+        }
+    }
+    __device__ __forceinline__ int column(int i) const { return head + (t + GROUP * i) * P::kWide; }
+    __device__ __forceinline__ bool some(int i) const { return column(i) < end; }
+    // kScalar: the second value of a pair may lie behind the row
+    __device__ __forceinline__ bool one(int i) const { return MODE == kScalar && column(i) + 1 >= end; }
+    __device__ __forceinline__ bool has_extra() const { return MODE == kShifted && extra >= 0; }
+
+    __device__ __forceinline__ void load(P &p, const T *row, int i) const { p.load(row + column(i), end - column(i)); }
+    __device__ __forceinline__ void store(const P &p, T *row, int i) const { p.store(row + column(i), end - column(i)); }
+    // the parameters of piece i
+    template <typename W>
+    __device__ __forceinline__ void params(const W *w, int i, Pair<Acc<T>> (&v)[P::kPairs]) const {
+        using A = Acc<T>;
+        if constexpr (MODE == kAligned) {
+            load_params<T>(w + column(i), v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < P::kPairs; ++j)
+                v[j] = {A(to_acc(w[column(i) + 2 * j])), one(i) ? A(0) : A(to_acc(w[column(i) + 2 * j + 1]))};
+        }
+    }
+};
+
+// kShifted: the parameters of a thread's columns lie in shared memory, as the
+// thread will read them.
+template <typename T, int GROUP, int N, int MODE>
+constexpr size_t forward_smem() {
+    return MODE == kShifted ? (size_t)threads_of(GROUP) * N * sizeof(Acc<T>) * 2 : 0;
+}
+
+template <typename T, typename W, int GROUP, int N, int MODE>
 __global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, sizeof(T)))
     k_layer_norm(const T *__restrict__ x, const W *__restrict__ w, const W *__restrict__ b,
                  int64_t rows, int64_t d, Acc<T> eps, T *__restrict__ y, Acc<T> *__restrict__ mean,
                  Acc<T> *__restrict__ rstd) {
     using A = Acc<T>;
-    using P = Piece<T, VEC>;
-    constexpr int kGroups = threads_of(GROUP) / GROUP, kPieces = N / P::kWide;
-    __shared__ A smem[2][threads_of(GROUP) / 32];
+    using P = Piece<T, MODE != kScalar>;
+    constexpr int kThreads = threads_of(GROUP), kGroups = kThreads / GROUP, kPieces = N / P::kWide;
+    __shared__ A smem[2][kThreads / 32];
+    extern __shared__ __align__(16) unsigned char raw[];
+    Pair<A> *params = reinterpret_cast<Pair<A> *>(raw);  // [w, b][piece][pair][thread]
     int turn = 0;
-    const int t = threadIdx.x % GROUP;
-    auto column = [&](int i) { return (t + GROUP * i) * P::kWide; };
+    // (kShifted: the host gives a number of groups that keeps each to one shift)
     const int64_t stride = (int64_t)gridDim.x * kGroups, first = (int64_t)blockIdx.x * kGroups;
-    const A inv = A(1) / A(d);
-    P next[kPieces];
     int64_t row = first + threadIdx.x / GROUP;
-    auto fetch = [&](int64_t r) {
-        if (r < rows)
+    const Columns<T, GROUP, MODE> c(row, d);
+    const A inv = A(1) / A(d);
+    A extra_w = 1, extra_b = 0;
+    if constexpr (MODE == kShifted) {
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-                if (column(i) < d) next[i].load(x + r * d + column(i), d - column(i));
+        for (int i = 0; i < kPieces; ++i) {
+            if (!c.some(i)) continue;
+            Pair<A> p[P::kPairs];
+            for (int which = 0; which < 2; ++which) {
+                const W *from = which ? b : w;
+                if (!from) continue;
+                c.params(from, i, p);
+#pragma unroll
+                for (int j = 0; j < P::kPairs; ++j)
+                    params[((which * kPieces + i) * P::kPairs + j) * kThreads + threadIdx.x] = p[j];
+            }
+        }
+        if (c.has_extra()) {
+            if (w) extra_w = to_acc(w[c.extra]);
+            if (b) extra_b = to_acc(b[c.extra]);
+        }
+    }
+    auto param = [&](const W *from, int which, int i, Pair<A>(&p)[P::kPairs]) {
+        if constexpr (MODE == kShifted) {
+#pragma unroll
+            for (int j = 0; j < P::kPairs; ++j)
+                p[j] = params[((which * kPieces + i) * P::kPairs + j) * kThreads + threadIdx.x];
+        } else {
+            c.params(from, i, p);
+        }
+    };
+    P next[kPieces];
+    T next_extra = from_acc<T>(0);
+    auto fetch = [&](int64_t r) {
+        if (r >= rows) return;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            if (c.some(i)) c.load(next[i], x + r * d, i);
+        if (c.has_extra()) next_extra = x[r * d + c.extra];
     };
     fetch(row);
     // whole groups take part in the block's barriers even behind the last row
     for (int64_t r0 = first; r0 < rows; r0 += stride, row += stride) {
+        const bool live = row < rows;
         Pair<A> v[kPieces][P::kPairs];
         Pair<A> s = both(A(0));
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const bool in = column(i) < d && row < rows;
+            const bool some = c.some(i) && live;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
-                v[i][j] = in ? next[i].get(j) : both(A(0));
+                v[i][j] = some ? next[i].get(j) : both(A(0));
                 s = s + v[i][j];
             }
         }
+        A extra = 0;
+        if (c.has_extra() && live) s.x += extra = to_acc(next_extra);
         fetch(row + stride);
         A sum[1] = {s.x + s.y};
         group_sums<GROUP>(sum, smem, turn);
@@ -208,39 +288,41 @@ __global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, 
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-            for (int j = 0; j < P::kPairs; ++j) {
-                v[i][j] = v[i][j] + both(-mu);
-                if (!VEC && column(i) + 1 >= d) v[i][j].y = 0;
-                if (column(i) < d) s = fma(v[i][j], v[i][j], s);
-            }
+            for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] + both(-mu);
+            if (!c.some(i)) continue;
+            if (c.one(i)) v[i][0].y = 0;
+#pragma unroll
+            for (int j = 0; j < P::kPairs; ++j) s = fma(v[i][j], v[i][j], s);
         }
+        extra -= mu;
+        if (c.has_extra()) s.x += extra * extra;
         sum[0] = s.x + s.y;
         group_sums<GROUP>(sum, smem, turn);
         const A rs = A(1) / sqrt(sum[0] * inv + eps);
-        if (row >= rows) continue;
+        if (!live) continue;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int e = column(i);
-            if (e >= d) continue;
+            if (!c.some(i)) continue;
             Pair<A> p[P::kPairs];
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * both(rs);
             if (w) {
-                load_params<T, VEC>(w + e, d - e, p);
+                param(w, 0, i, p);
 #pragma unroll
                 for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] * p[j];
             }
             if (b) {
-                load_params<T, VEC>(b + e, d - e, p);
+                param(b, 1, i, p);
 #pragma unroll
                 for (int j = 0; j < P::kPairs; ++j) v[i][j] = v[i][j] + p[j];
             }
             P o;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) o.set(j, v[i][j]);
-            o.store(y + row * d + e, d - e);
+            c.store(o, y + row * d, i);
         }
-        if (t == 0) {
+        if (c.has_extra()) y[row * d + c.extra] = from_acc<T>(extra * rs * extra_w + extra_b);
+        if (c.t == 0) {
             if (mean) mean[row] = mu;
             if (rstd) rstd[row] = rs;
         }
@@ -264,57 +346,67 @@ __host__ __device__ constexpr int ring_stages() {
     constexpr int n = 196608 / backward_resident(GROUP, N, sizeof(T)) / bytes;
     return n > 4 ? 4 : n;
 }
-template <typename T, int GROUP, int N, bool VEC>
+template <typename T, int GROUP, int N, int MODE>
 constexpr size_t backward_smem() {
     // the ring, or the columns where the block's groups meet at the end
-    const size_t ring = VEC ? (size_t)ring_stages<T, GROUP, N>() * threads_of(GROUP) * 2 * N * sizeof(T) : 0;
+    const size_t ring = MODE != kScalar ? (size_t)ring_stages<T, GROUP, N>() * threads_of(GROUP) * 2 * N * sizeof(T) : 0;
     const size_t columns = GROUP < threads_of(GROUP) ? (size_t)GROUP * N * sizeof(Acc<T>) : 0;
     return ring > columns ? ring : columns;
 }
+// kShifted: this many blocks share a run of rows, so that each group's rows have
+// one shift.
+template <typename T>
+__host__ __device__ constexpr int shift_blocks(int groups) {
+    return 16 / (int)sizeof(T) > groups ? 16 / (int)sizeof(T) / groups : 1;
+}
 
-// partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows,
-// which are consecutive
-template <typename T, typename W, int GROUP, int N, bool VEC>
+// partial: [gridDim.x][2][d], sums of dy * xhat and of dy over the block's rows, a
+// consecutive run (or every shift_blocks-th of one)
+template <typename T, typename W, int GROUP, int N, int MODE>
 __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N, sizeof(T)))
     k_layer_norm_backward(const T *__restrict__ dy, const T *__restrict__ x,
                           const Acc<T> *__restrict__ mean, const Acc<T> *__restrict__ rstd,
                           const W *__restrict__ w, int64_t rows, int64_t d, T *__restrict__ dx,
                           Acc<T> *__restrict__ partial) {
     using A = Acc<T>;
-    using P = Piece<T, VEC>;
+    using P = Piece<T, MODE != kScalar>;
     constexpr int kThreads = threads_of(GROUP), kGroups = kThreads / GROUP, kPieces = N / P::kWide;
     constexpr int kStages = ring_stages<T, GROUP, N>();
+    constexpr int kShare = MODE == kShifted ? shift_blocks<T>(kGroups) : 1, kStep = kShare * kGroups;
     __shared__ A smem[2][2 * (kThreads / 32)];
     extern __shared__ __align__(16) unsigned char raw[];
-    A *columns = reinterpret_cast<A *>(raw);       // [GROUP * N], after the rows
+    A *columns = reinterpret_cast<A *>(raw);       // [d], after the rows
     uint4 *ring = reinterpret_cast<uint4 *>(raw);  // [stage][x, dy][piece][thread]
     int turn = 0;
-    const int t = threadIdx.x % GROUP;
-    auto column = [&](int i) { return (t + GROUP * i) * P::kWide; };
-    const int64_t begin = rows * blockIdx.x / gridDim.x, end = rows * (blockIdx.x + 1) / gridDim.x;
+    const int64_t run = blockIdx.x / kShare, runs = gridDim.x / kShare;
+    const int64_t begin = rows * run / runs, end = rows * (run + 1) / runs;
+    const int count = (int)(end - begin), lead = (int)(blockIdx.x % kShare * kGroups + threadIdx.x / GROUP);
+    const int64_t mine = begin + lead;  // this thread's first row
+    const Columns<T, GROUP, MODE> c(mine, d);
     Pair<A> aw[kPieces][P::kPairs], ab[kPieces][P::kPairs], wv[kPieces][P::kPairs];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
         for (int j = 0; j < P::kPairs; ++j) aw[i][j] = ab[i][j] = both(A(0)), wv[i][j] = both(A(1));
-        if (w && column(i) < d) load_params<T, VEC>(w + column(i), d - column(i), wv[i]);
+        if (w && c.some(i)) c.params(w, i, wv[i]);
     }
-    // this thread's first value in its next row to fetch, and in the row at hand
-    const int64_t mine = begin + threadIdx.x / GROUP, step = kGroups * d;
-    const int count = (int)(end - begin), lead = (int)(threadIdx.x / GROUP);
-    int64_t fetched = mine * d + t * P::kWide, at = fetched;
+    const A extra_w = w && c.has_extra() ? to_acc(w[c.extra]) : A(1);
+    A extra_aw = 0, extra_ab = 0;
+    // values to the next row to fetch, and to the row at hand
+    const int64_t step = kStep * d;
+    int64_t fetched = mine * d, at = fetched;
     constexpr uint32_t kStageBytes = 2 * kPieces * kThreads * 16, kRing = kStages * kStageBytes;
     const uint32_t slot0 = smem_addr(ring + threadIdx.x);
     uint32_t into = 0, from = 0;  // bytes into the ring
     auto fetch = [&](int i_row) {
-        if constexpr (VEC) {
+        if constexpr (MODE != kScalar) {
             if (i_row < count)
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    if (column(i) >= d) continue;
+                    if (!c.some(i)) continue;
                     const uint32_t slot = slot0 + into + i * kThreads * 16;
-                    cp_async<16>(slot, x + fetched + GROUP * i * P::kWide);
-                    cp_async<16>(slot + kPieces * kThreads * 16, dy + fetched + GROUP * i * P::kWide);
+                    cp_async<16>(slot, x + fetched + c.column(i));
+                    cp_async<16>(slot + kPieces * kThreads * 16, dy + fetched + c.column(i));
                 }
             cp_async_commit();  // an empty group where there is no row: the count stays
             fetched += step;
@@ -322,15 +414,17 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
         }
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(lead + i * kGroups);
+    for (int i = 0; i < kStages - 1; ++i) fetch(lead + i * kStep);
     const A *mu_at = mean + mine, *rs_at = rstd + mine;
     const A inv = A(1) / A(d);
     A next_mu = lead < count ? *mu_at : A(0), next_rs = lead < count ? *rs_at : A(0);
-    for (int r0 = 0; r0 < count; r0 += kGroups, at += step) {
+    T next_ex = from_acc<T>(0), next_eg = from_acc<T>(0);  // the extra column's x and dy
+    if (c.has_extra() && lead < count) next_ex = x[at + c.extra], next_eg = dy[at + c.extra];
+    for (int r0 = 0; r0 < count; r0 += kStep, at += step) {
         const bool live = r0 + lead < count;
         P hx[kPieces], hg[kPieces];
-        if constexpr (VEC) {
-            fetch(r0 + lead + (kStages - 1) * kGroups);  // into the stage that was read last time
+        if constexpr (MODE != kScalar) {
+            fetch(r0 + lead + (kStages - 1) * kStep);  // into the stage that was read last time
             cp_async_wait<kStages - 1>();
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
@@ -342,14 +436,15 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
         } else if (live) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                if (column(i) < d) {
-                    hx[i].load(x + at + GROUP * i * P::kWide, d - column(i));
-                    hg[i].load(dy + at + GROUP * i * P::kWide, d - column(i));
-                }
+                if (c.some(i)) c.load(hx[i], x + at, i), c.load(hg[i], dy + at, i);
         }
         const Pair<A> mu = both(-next_mu), rs = both(next_rs);
-        mu_at += kGroups, rs_at += kGroups;
-        if (r0 + lead + kGroups < count) next_mu = *mu_at, next_rs = *rs_at;
+        mu_at += kStep, rs_at += kStep;
+        const A ex = (to_acc(next_ex) - next_mu) * next_rs, eg = to_acc(next_eg), ev = eg * extra_w;
+        if (r0 + lead + kStep < count) {
+            next_mu = *mu_at, next_rs = *rs_at;
+            if (c.has_extra()) next_ex = x[at + step + c.extra], next_eg = dy[at + step + c.extra];
+        }
         Pair<A> s1 = both(A(0)), s2 = both(A(0));
         // bf16: kept as they are worked out (unpacking them again costs more
         // than the registers); else worked out again
@@ -357,7 +452,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
         Pair<A> xhat[kPieces][P::kPairs], v[kPieces][P::kPairs];
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            if (column(i) >= d || !live) continue;
+            if (!c.some(i) || !live) continue;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
                 const Pair<A> g = hg[i].get(j);
@@ -369,6 +464,12 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
                 s2 = fma(v[i][j], xhat[i][j], s2);
             }
         }
+        if (c.has_extra() && live) {
+            extra_aw += eg * ex;
+            extra_ab += eg;
+            s1.x += ev;
+            s2.x += ev * ex;
+        }
         A sums[2] = {s1.x + s1.y, s2.x + s2.y};
         group_sums<GROUP>(sums, smem, turn);
         s1 = both(-sums[0] * inv);
@@ -376,7 +477,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
         if (!live || !dx) continue;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            if (column(i) >= d) continue;
+            if (!c.some(i)) continue;
             P o;
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) {
@@ -386,41 +487,41 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
                 }
                 o.set(j, rs * fma(xhat[i][j], s2, v[i][j] + s1));
             }
-            o.store(dx + at + GROUP * i * P::kWide, d - column(i));
+            c.store(o, dx + at, i);
         }
+        if (c.has_extra()) dx[at + c.extra] = from_acc<T>(rs.x * (ex * s2.x + (ev + s1.x)));
     }
-    if constexpr (VEC) cp_async_wait<0>();
+    if constexpr (MODE != kScalar) cp_async_wait<0>();
     if (!partial) return;
-    // the block's groups one after the other, then the block's row of partials
+    // the block's groups one after the other (kShifted: each with columns of its
+    // own, so by column), then the block's row of partials
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         Pair<A>(&a)[kPieces][P::kPairs] = which ? ab : aw;
-        if constexpr (kGroups > 1) {
-            for (int g = 0; g < kGroups; ++g) {
-                __syncthreads();
-                if (threadIdx.x / GROUP != g) continue;
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-                    for (int j = 0; j < P::kPairs; ++j) {
-                        A *c = columns + column(i) + 2 * j;
-                        if (g > 0) a[i][j].x += c[0];
-                        c[0] = a[i][j].x;
-                        if (g > 0) a[i][j].y += c[1];
-                        c[1] = a[i][j].y;
-                    }
-            }
-            if (threadIdx.x / GROUP != kGroups - 1) continue;
-        }
         A *out = partial + (blockIdx.x * 2 + which) * d;
+        for (int g = 0; g < kGroups; ++g) {
+            if constexpr (kGroups > 1) __syncthreads();
+            if (threadIdx.x / GROUP != g) continue;
+            const bool last = g == kGroups - 1;
+            // (loads first: the compiler cannot tell them from the stores)
+            A sum[kPieces][P::kWide];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            if (column(i) >= d) continue;
+            for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-            for (int j = 0; j < P::kPairs; ++j) {
-                out[column(i) + 2 * j] = a[i][j].x;
-                if (VEC || column(i) + 1 < d) out[column(i) + 2 * j + 1] = a[i][j].y;
+                for (int j = 0; j < P::kWide; ++j) {
+                    sum[i][j] = j & 1 ? a[i][j / 2].y : a[i][j / 2].x;
+                    if (kGroups > 1 && g > 0 && c.some(i) && !(j && c.one(i))) sum[i][j] += columns[c.column(i) + j];
+                }
+            A *to = last ? out : columns;
+            if (c.has_extra()) {
+                const A mine_extra = which ? extra_ab : extra_aw;
+                to[c.extra] = kGroups > 1 && g > 0 ? mine_extra + columns[c.extra] : mine_extra;
             }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int j = 0; j < P::kWide; ++j)
+                    if (c.some(i) && !(j && c.one(i))) to[c.column(i) + j] = sum[i][j];
         }
     }
 }
@@ -553,15 +654,17 @@ struct Shape {
     int group, values;
 };
 Shape shape_of(int64_t d, int dtype) {
+    // (16 threads at least where up to 14 values lie beside a row's pieces)
+    const bool beside = dtype == BGL_BF16 && d % 8;
     const int most = dtype == BGL_F64 ? 8 : 16;
-    if (d <= 8 * 8) return {8, 8};
+    if (d <= 8 * 8 && !beside) return {8, 8};
     if (d <= 16 * 8) return {16, 8};
     if (d <= 32 * 8) return {32, 8};
     int group = 32;
     while ((int64_t)group * most < d) group *= 2;
     return {group, most};
 }
-int64_t most_held(int dtype) { return dtype == BGL_F64 ? kMostHeld / 2 : kMostHeld; }
+bool is_held(int64_t d, int dtype) { return d <= (dtype == BGL_F64 ? kMostHeld / 2 : kMostHeld); }
 
 // Blocks of the backward pass, one partial row each: resident ones, a fixed
 // number for a given device so that the sums keep their order.
@@ -570,10 +673,11 @@ int64_t backward_blocks(int64_t rows, int64_t d, int dtype) {
     const int groups = threads_of(shape.group) / shape.group;
     const int resident = backward_resident(shape.group, shape.values, (int)row_elem_size(dtype));
     const int64_t want = (rows + groups - 1) / groups, most = (int64_t)num_sms() * resident;
-    return want < most ? want : most;
+    // whole runs of the blocks that share one (shift_blocks: at most 8)
+    return want < most ? (want + 7) / 8 * 8 : most / 8 * 8;
 }
 int64_t parts_of(int64_t rows, int64_t d, int dtype) {
-    return d <= most_held(dtype) ? backward_blocks(rows, d, dtype) : splits_of(rows);
+    return is_held(d, dtype) ? backward_blocks(rows, d, dtype) : splits_of(rows);
 }
 
 int check_norm(const char *who, int64_t rows, int64_t d, int dtype, int wdtype) {
@@ -602,6 +706,14 @@ int with_shape(Shape s, F &&f) {
     return f(Constant<512, M>());
 }
 
+// Rows of whole 16-byte pieces, of shifted ones, or (where an array does not begin
+// on 16 bytes) of single values.
+template <typename T>
+RowMode row_mode(int64_t d, bool arrays, bool params) {
+    if (!arrays) return kScalar;
+    return d * sizeof(T) % 16 == 0 && params ? kAligned : kShifted;
+}
+
 struct Forward {
     const void *x, *w, *b;
     int64_t rows, d;
@@ -617,24 +729,32 @@ int forward(const Forward &p) {
     const W *w = (const W *)p.w, *b = (const W *)p.b;
     T *y = (T *)p.y;
     A *mean = (A *)p.mean, *rstd = (A *)p.rstd;
-    if (p.d > most_held(p.dtype)) {
+    if (!is_held(p.d, p.dtype)) {
         const int64_t cap = (int64_t)num_sms() * 8;
         k_layer_norm_long<T, W><<<(unsigned)(p.rows < cap ? p.rows : cap), kThreads, 0, p.s>>>(
             x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
         BGL_LAUNCH_CHECK();
         return BGL_OK;
     }
-    const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(y, 16) && aligned(w, 16) && aligned(b, 16);
+    const RowMode mode = row_mode<T>(p.d, aligned(x, 16) && aligned(y, 16), aligned(w, 16) && aligned(b, 16));
     return with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
         constexpr int G = decltype(c)::group, N = decltype(c)::values, threads = threads_of(G), per = threads / G;
         // one wave of resident blocks (888 blocks where 592 are resident: 38 us
         // for 8192 x 4096 bf16, against 33 us)
         const int64_t want = (p.rows + per - 1) / per, cap = (int64_t)num_sms() * forward_resident(G, N, sizeof(T));
-        const unsigned grid = (unsigned)(want < cap ? want : cap);
-        if (vec)
-            k_layer_norm<T, W, G, N, true><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
-        else
-            k_layer_norm<T, W, G, N, false><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+        // (a multiple of 8 blocks keeps every group to rows of one shift)
+        const unsigned grid = (unsigned)(want < cap ? want : cap / 8 * 8);
+        if (mode == kAligned) {
+            k_layer_norm<T, W, G, N, kAligned><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+        } else if (mode == kShifted) {
+            constexpr size_t smem = forward_smem<T, G, N, kShifted>();
+            if (smem > 48 * 1024)
+                BGL_CUDA(cudaFuncSetAttribute(k_layer_norm<T, W, G, N, kShifted>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            k_layer_norm<T, W, G, N, kShifted><<<grid, threads, smem, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+        } else {
+            k_layer_norm<T, W, G, N, kScalar><<<grid, threads, 0, p.s>>>(x, w, b, p.rows, p.d, (A)p.eps, y, mean, rstd);
+        }
         BGL_LAUNCH_CHECK();
         return (int)BGL_OK;
     });
@@ -658,7 +778,7 @@ int backward(const Backward &p) {
     const int64_t parts = parts_of(p.rows, p.d, p.dtype);
     Carver carver(p.ws);
     A *partial = sums ? carver.take<A>((size_t)(2 * parts * p.d)) : nullptr;
-    if (p.rows && p.d > most_held(p.dtype)) {
+    if (p.rows && !is_held(p.d, p.dtype)) {
         const int64_t cap = (int64_t)num_sms() * 8;
         if (dx) {
             k_layer_norm_dx_long<T, W><<<(unsigned)(p.rows < cap ? p.rows : cap), kThreads, 0, p.s>>>(
@@ -672,21 +792,20 @@ int backward(const Backward &p) {
             BGL_LAUNCH_CHECK();
         }
     } else if (p.rows && (dx || sums)) {
-        const bool vec = p.d * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) && aligned(w, 16);
+        const RowMode mode = row_mode<T>(p.d, aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16), aligned(w, 16));
         const int rc = with_shape<T>(shape_of(p.d, p.dtype), [&](auto c) {
             constexpr int G = decltype(c)::group, N = decltype(c)::values, threads = threads_of(G);
             const unsigned grid = (unsigned)parts;
-            constexpr size_t smem = backward_smem<T, G, N, true>(), plain = backward_smem<T, G, N, false>();
-            if (vec) {
+            auto launch = [&](auto kernel, size_t smem) {
                 if (smem > 48 * 1024)
-                    BGL_CUDA(cudaFuncSetAttribute(k_layer_norm_backward<T, W, G, N, true>,
-                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-                k_layer_norm_backward<T, W, G, N, true><<<grid, threads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
-            } else {
-                k_layer_norm_backward<T, W, G, N, false><<<grid, threads, plain, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
-            }
-            BGL_LAUNCH_CHECK();
-            return (int)BGL_OK;
+                    BGL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                kernel<<<grid, threads, smem, p.s>>>(dy, x, mean, rstd, w, p.rows, p.d, dx, partial);
+                BGL_LAUNCH_CHECK();
+                return (int)BGL_OK;
+            };
+            if (mode == kAligned) return launch(k_layer_norm_backward<T, W, G, N, kAligned>, backward_smem<T, G, N, kAligned>());
+            if (mode == kShifted) return launch(k_layer_norm_backward<T, W, G, N, kShifted>, backward_smem<T, G, N, kShifted>());
+            return launch(k_layer_norm_backward<T, W, G, N, kScalar>, backward_smem<T, G, N, kScalar>());
         });
         if (rc) return rc;
     }

@@ -29,6 +29,12 @@ __device__ __forceinline__ double from_acc<double>(double x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_acc<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// How rows are moved: by single values; in whole 16-byte pieces; or, where their
+// length is no multiple of 16 bytes, in the aligned pieces inside them and the few
+// values beside those one by one.  Which values that are is the same for all rows
+// of one remainder modulo the values of a piece.
+enum RowMode { kScalar = 0, kAligned = 1, kShifted = 2 };
+
 template <typename A>
 __device__ __forceinline__ A warp_sum(A v) {
 #pragma unroll
