@@ -346,12 +346,18 @@ __host__ __device__ constexpr int ring_stages() {
     constexpr int n = 196608 / backward_resident(GROUP, N, sizeof(T)) / bytes;
     return n > 4 ? 4 : n;
 }
+// kShifted: the weights of a thread's columns lie in shared memory, as the thread
+// will read them (registers are short with the extra column's values beside).
+template <typename T, int GROUP, int N, int MODE>
+__host__ __device__ constexpr size_t backward_weights() {
+    return MODE == kShifted ? (size_t)threads_of(GROUP) * N * sizeof(Acc<T>) : 0;
+}
 template <typename T, int GROUP, int N, int MODE>
 constexpr size_t backward_smem() {
     // the ring, or the columns where the block's groups meet at the end
     const size_t ring = MODE != kScalar ? (size_t)ring_stages<T, GROUP, N>() * threads_of(GROUP) * 2 * N * sizeof(T) : 0;
     const size_t columns = GROUP < threads_of(GROUP) ? (size_t)GROUP * N * sizeof(Acc<T>) : 0;
-    return ring > columns ? ring : columns;
+    return (ring > columns ? ring : columns) + backward_weights<T, GROUP, N, MODE>();
 }
 // kShifted: this many blocks share a run of rows, so that each group's rows have
 // one shift.
@@ -375,20 +381,32 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
     constexpr int kShare = MODE == kShifted ? shift_blocks<T>(kGroups) : 1, kStep = kShare * kGroups;
     __shared__ A smem[2][2 * (kThreads / 32)];
     extern __shared__ __align__(16) unsigned char raw[];
-    A *columns = reinterpret_cast<A *>(raw);       // [d], after the rows
-    uint4 *ring = reinterpret_cast<uint4 *>(raw);  // [stage][x, dy][piece][thread]
+    constexpr size_t kWeights = backward_weights<T, GROUP, N, MODE>();
+    Pair<A> *weights = reinterpret_cast<Pair<A> *>(raw);      // kShifted: [piece][pair][thread]
+    A *columns = reinterpret_cast<A *>(raw + kWeights);       // [d], after the rows
+    uint4 *ring = reinterpret_cast<uint4 *>(raw + kWeights);  // [stage][x, dy][piece][thread]
     int turn = 0;
     const int64_t run = blockIdx.x / kShare, runs = gridDim.x / kShare;
     const int64_t begin = rows * run / runs, end = rows * (run + 1) / runs;
     const int count = (int)(end - begin), lead = (int)(blockIdx.x % kShare * kGroups + threadIdx.x / GROUP);
     const int64_t mine = begin + lead;  // this thread's first row
     const Columns<T, GROUP, MODE> c(mine, d);
-    Pair<A> aw[kPieces][P::kPairs], ab[kPieces][P::kPairs], wv[kPieces][P::kPairs];
+    Pair<A> aw[kPieces][P::kPairs], ab[kPieces][P::kPairs];
+    Pair<A> wv[MODE == kShifted ? 1 : kPieces][P::kPairs];
+    auto weight = [&](int i, int j) {
+        return MODE == kShifted ? weights[(i * P::kPairs + j) * kThreads + threadIdx.x] : wv[MODE == kShifted ? 0 : i][j];
+    };
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-        for (int j = 0; j < P::kPairs; ++j) aw[i][j] = ab[i][j] = both(A(0)), wv[i][j] = both(A(1));
-        if (w && c.some(i)) c.params(w, i, wv[i]);
+        for (int j = 0; j < P::kPairs; ++j) {
+            aw[i][j] = ab[i][j] = both(A(0));
+            wv[MODE == kShifted ? 0 : i][j] = both(A(1));
+        }
+        if (w && c.some(i)) c.params(w, i, wv[MODE == kShifted ? 0 : i]);
+        if constexpr (MODE == kShifted)
+#pragma unroll
+            for (int j = 0; j < P::kPairs; ++j) weights[(i * P::kPairs + j) * kThreads + threadIdx.x] = wv[0][j];
     }
     const A extra_w = w && c.has_extra() ? to_acc(w[c.extra]) : A(1);
     A extra_aw = 0, extra_ab = 0;
@@ -457,7 +475,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
             for (int j = 0; j < P::kPairs; ++j) {
                 const Pair<A> g = hg[i].get(j);
                 xhat[i][j] = (hx[i].get(j) + mu) * rs;
-                v[i][j] = g * wv[i][j];
+                v[i][j] = g * weight(i, j);
                 aw[i][j] = fma(g, xhat[i][j], aw[i][j]);
                 ab[i][j] = ab[i][j] + g;
                 s1 = s1 + v[i][j];
@@ -483,7 +501,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
             for (int j = 0; j < P::kPairs; ++j) {
                 if constexpr (!kKeep) {
                     xhat[i][j] = (hx[i].get(j) + mu) * rs;
-                    v[i][j] = hg[i].get(j) * wv[i][j];
+                    v[i][j] = hg[i].get(j) * weight(i, j);
                 }
                 o.set(j, rs * fma(xhat[i][j], s2, v[i][j] + s1));
             }
