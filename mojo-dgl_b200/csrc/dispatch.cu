@@ -189,6 +189,155 @@ struct Piece {
     }
 };
 
+// A row whose length is no multiple of 16 bytes, seen from the array it is written
+// to: the aligned pieces inside it, and the values before and behind them.
+template <typename T>
+struct Inside {
+    using P = Piece<T, true>;
+    int64_t head, end, d;  // first value of the pieces, and the one behind them
+    __device__ __forceinline__ Inside(int64_t row, int64_t d_) : d(d_) {
+        head = (int64_t)(-(uint64_t)(row * d_) % P::kWide);
+        if (head > d) head = d;
+        end = head + (d - head) / P::kWide * P::kWide;
+    }
+    __device__ __forceinline__ int beside() const { return (int)(head + d - end); }
+    __device__ __forceinline__ int64_t value(int i) const { return i < head ? i : end + i - head; }
+};
+
+// 16 bytes from any address: two aligned pieces, shifted into one once they are
+// there.  `stop` is the end of the array; a piece that reached beyond it is put
+// together from values.
+template <typename T>
+struct AnyPiece {
+    uint4 lo, hi;
+    unsigned shift;
+
+    __device__ __forceinline__ void fetch(const T *from, const T *stop) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+        const uint4 *a = reinterpret_cast<const uint4 *>(at & ~uintptr_t(15));
+        shift = (unsigned)(at & 15);
+        if (reinterpret_cast<const T *>(a + 2) > stop) {
+            Piece<T, true> p;
+#pragma unroll
+            for (int i = 0; i < Piece<T, true>::kWide; ++i) p.v[i] = from[i];
+            lo = p.raw;
+            shift = 0;
+        } else {
+            lo = __ldg(a);
+            if (shift) hi = __ldg(a + 1);
+        }
+    }
+    __device__ __forceinline__ Piece<T, true> get() const {
+        Piece<T, true> p;
+        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (shift & 8)
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+        if (shift & 4)
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+        if (sizeof(T) == 2) {
+            const unsigned bits = (shift & 3) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+        }
+        p.raw = make_uint4(w[0], w[1], w[2], w[3]);
+        return p;
+    }
+};
+// Brings a row towards the SM before it is known which of its pieces are wanted.
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T *row, int64_t d, int thread, int threads) {
+    for (int64_t e = thread * (128 / (int)sizeof(T)); e < d; e += threads * (128 / (int)sizeof(T)))
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(row + e));
+}
+
+// Rows of odd lengths (kShifted): as the kernels below, in the pieces of what is
+// written; what is read lies at any shift to them.  20000 x 2 rows of 1023 bf16
+// values: dispatch 81 -> 49 us, combine 84 -> 41, its gradient 88 -> 52 against
+// single values.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    k_dispatch_odd(const T *__restrict__ x, const int32_t *__restrict__ positions, int64_t tokens,
+                   int k, int64_t d, T *__restrict__ rows) {
+    using P = Piece<T, true>;
+    const int64_t t = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    const T *from = x + t * d, *stop = x + tokens * d;
+    prefetch_row(from, d, threadIdx.x, blockDim.x);
+#pragma unroll 2
+    for (int j = 0; j < k; ++j) {
+        int64_t row;
+        const bool sent = row_of(__ldg(positions + t * k + j), tokens * k, row);
+        if (row < 0) continue;
+        const Inside<T> in(row, d);
+        T *to = rows + row * d;
+        for (int64_t e = in.head + threadIdx.x * P::kWide; e < in.end; e += blockDim.x * P::kWide) {
+            P v;
+            v.zero();
+            if (sent) {
+                AnyPiece<T> any;
+                any.fetch(from + e, stop);
+                v = any.get();
+            }
+            v.store(to + e);
+        }
+        for (int i = threadIdx.x; i < in.beside(); i += blockDim.x)
+            to[in.value(i)] = sent ? from[in.value(i)] : from_acc<T>(0);
+    }
+}
+
+template <typename T, int kFlight>
+__global__ void __launch_bounds__(kThreads)
+    k_combine_odd(const T *__restrict__ rows, const int32_t *__restrict__ positions,
+                  const Acc<T> *__restrict__ weights, int64_t tokens, int k, int64_t d,
+                  T *__restrict__ y) {
+    using A = Acc<T>;
+    using P = Piece<T, true>;
+    const int64_t t = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
+    if (t >= tokens) return;
+    const Inside<T> in(t, d);
+    const T *stop = rows + tokens * k * d;
+    T *to = y + t * d;
+    // a value beside the pieces goes along with a thread's first piece (there are
+    // fewer of them than threads with a piece)
+    int64_t extra = (int)threadIdx.x < in.beside() ? in.value(threadIdx.x) : -1;
+    for (int64_t e = in.head + threadIdx.x * P::kWide; e < in.end; e += blockDim.x * P::kWide, extra = -1) {
+        A sum[P::kWide], extra_sum = 0;
+#pragma unroll
+        for (int i = 0; i < P::kWide; ++i) sum[i] = 0;
+        for (int j0 = 0; j0 < k; j0 += kFlight) {  // rows under way
+            AnyPiece<T> any[kFlight];
+            T beside[kFlight];
+            A w[kFlight];
+            bool sent[kFlight];
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j) {
+                int64_t row;
+                sent[j] = j0 + j < k && row_of(__ldg(positions + t * k + j0 + j), tokens * k, row);
+                if (sent[j]) {
+                    any[j].fetch(rows + row * d + e, stop);
+                    if (extra >= 0) beside[j] = rows[row * d + extra];
+                    w[j] = weights ? __ldg(weights + t * k + j0 + j) : A(1);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kFlight; ++j) {
+                if (!sent[j]) continue;
+                const P v = any[j].get();
+#pragma unroll
+                for (int i = 0; i < P::kWide; ++i) sum[i] += w[j] * to_acc(v.v[i]);
+                if (extra >= 0) extra_sum += w[j] * to_acc(beside[j]);
+            }
+        }
+        P o;
+#pragma unroll
+        for (int i = 0; i < P::kWide; ++i) o.v[i] = from_acc<T>(sum[i]);
+        o.store(to + e);
+        if (extra >= 0) to[extra] = from_acc<T>(extra_sum);
+    }
+}
+
 // blockDim.x threads over a row's pieces, blockDim.y tokens.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
@@ -310,6 +459,66 @@ __global__ void __launch_bounds__(backward_threads(GROUP))
     }
 }
 
+// The same by GROUP threads a token for rows of odd lengths, a choice at a time.
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(backward_threads(GROUP))
+    k_combine_backward_odd(const T *__restrict__ dy, const T *__restrict__ rows,
+                           const int32_t *__restrict__ positions, const Acc<T> *__restrict__ weights,
+                           int64_t tokens, int k, int64_t d, T *__restrict__ drows,
+                           Acc<T> *__restrict__ dweights) {
+    using A = Acc<T>;
+    using P = Piece<T, true>;
+    __shared__ A smem[32];
+    const int own = threadIdx.x % GROUP;
+    const int64_t t = blockIdx.x * (int64_t)(backward_threads(GROUP) / GROUP) + threadIdx.x / GROUP;
+    if (t >= tokens) return;  // whole groups; a group of a block is the block
+    const T *from = dy + t * d, *stop = dy + tokens * d;
+    prefetch_row(from, d, own, GROUP);
+    for (int j = 0; j < k; ++j) {
+        int64_t row;
+        const bool sent = row_of(__ldg(positions + t * k + j), tokens * k, row);
+        const A w = !sent ? A(0) : weights ? __ldg(weights + t * k + j) : A(1);
+        const bool dots = dweights && sent;
+        A dot = 0;
+        if (row >= 0) {
+            const Inside<T> in(row, d);
+            const T *with = rows + row * d;
+            T *to = drows + row * d;
+            // the value beside the pieces (at most one a thread) is under way with them
+            const int64_t extra = own < in.beside() ? in.value(own) : -1;
+            T extra_g = from_acc<T>(0), extra_v = from_acc<T>(0);
+            if (extra >= 0) {
+                extra_g = from[extra];
+                if (dots) extra_v = with[extra];
+            }
+#pragma unroll 2
+            for (int64_t e = in.head + own * P::kWide; e < in.end; e += GROUP * P::kWide) {
+                AnyPiece<T> any;
+                any.fetch(from + e, stop);
+                P v, o;
+                if (dots) v.load(with + e);
+                const P g = any.get();
+#pragma unroll
+                for (int i = 0; i < P::kWide; ++i) {
+                    const A gi = to_acc(g.v[i]);
+                    if (dots) dot += gi * to_acc(v.v[i]);
+                    o.v[i] = from_acc<T>(sent ? w * gi : A(0));
+                }
+                if (drows) o.store(to + e);
+            }
+            if (extra >= 0) {
+                const A gi = to_acc(extra_g);
+                if (dots) dot += gi * to_acc(extra_v);
+                if (drows) to[extra] = from_acc<T>(sent ? w * gi : A(0));
+            }
+        }
+        if (dweights) {
+            const A sum = GROUP == 32 ? warp_sum(dot) : block_sum(dot, smem);
+            if (own == 0) dweights[t * k + j] = sum;
+        }
+    }
+}
+
 int check_rows(const char *who, int64_t tokens, int64_t k, int64_t d, int dtype) {
     if (!row_dtype(dtype)) return fail(BGL_E_UNSUPPORTED, "%s: dtype %d", who, dtype);
     if (tokens < 0 || k < 0 || d < 0) return fail(BGL_E_INVALID, "%s: negative size", who);
@@ -325,9 +534,12 @@ dim3 row_block(int64_t pieces) {
     while (x < pieces && x < kThreads) x *= 2;
     return dim3(x, kThreads / x);
 }
+// (below 16 pieces a row, what is beside them costs more than the pieces save)
 template <typename T>
-bool pieces_of_16(int64_t d, const void *a, const void *b, const void *c = nullptr) {
-    return d * sizeof(T) % 16 == 0 && aligned(a, 16) && aligned(b, 16) && aligned(c, 16);
+RowMode row_mode(int64_t d, const void *a, const void *b, const void *c = nullptr) {
+    if (!aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16)) return kScalar;
+    if (d * sizeof(T) % 16 == 0) return kAligned;
+    return d * sizeof(T) >= 256 ? kShifted : kScalar;
 }
 unsigned token_blocks(int64_t tokens, unsigned per) { return (unsigned)((tokens + per - 1) / per); }
 
@@ -342,40 +554,49 @@ struct Rows {
 };
 template <typename T>
 int dispatch_as(const Rows &p) {
-    const bool vec = pieces_of_16<T>(p.d, p.in, p.out);
-    const dim3 block = row_block(vec ? p.d * (int64_t)sizeof(T) / 16 : p.d);
+    const RowMode mode = row_mode<T>(p.d, p.in, p.out);
+    const dim3 block = row_block(mode == kScalar ? p.d : p.d * (int64_t)sizeof(T) / 16);
     const unsigned grid = token_blocks(p.tokens, block.y);
-    if (vec) k_dispatch<T, true><<<grid, block, 0, p.s>>>((const T *)p.in, p.positions, p.tokens, p.k, p.d, (T *)p.out);
-    else k_dispatch<T, false><<<grid, block, 0, p.s>>>((const T *)p.in, p.positions, p.tokens, p.k, p.d, (T *)p.out);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    auto launch = [&](auto kernel) {
+        kernel<<<grid, block, 0, p.s>>>((const T *)p.in, p.positions, p.tokens, p.k, p.d, (T *)p.out);
+        BGL_LAUNCH_CHECK();
+        return (int)BGL_OK;
+    };
+    return mode == kAligned ? launch(k_dispatch<T, true>) : mode == kShifted ? launch(k_dispatch_odd<T>) : launch(k_dispatch<T, false>);
 }
 template <typename T>
 int combine_as(const Rows &p) {
-    using A = Acc<T>;
-    const bool vec = pieces_of_16<T>(p.d, p.rows, p.out);
-    const dim3 block = row_block(vec ? p.d * (int64_t)sizeof(T) / 16 : p.d);
+    RowMode mode = row_mode<T>(p.d, p.rows, p.out);
+    // values of 4 and 8 bytes move about as fast one by one as in pieces that have
+    // to be shifted (float32, 6 rows of 1031 a token: 72 us against 111; bf16: 72
+    // against 49)
+    if (mode == kShifted && sizeof(T) > 2) mode = kScalar;
+    const dim3 block = row_block(mode == kScalar ? p.d : p.d * (int64_t)sizeof(T) / 16);
     const unsigned grid = token_blocks(p.tokens, block.y);
-    const T *rows = (const T *)p.rows;
-    const A *w = (const A *)p.weights;
-    if (vec) k_combine<T, true><<<grid, block, 0, p.s>>>(rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out);
-    else k_combine<T, false><<<grid, block, 0, p.s>>>(rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    auto launch = [&](auto kernel) {
+        kernel<<<grid, block, 0, p.s>>>((const T *)p.rows, p.positions, (const Acc<T> *)p.weights, p.tokens, p.k, p.d, (T *)p.out);
+        BGL_LAUNCH_CHECK();
+        return (int)BGL_OK;
+    };
+    if (mode == kAligned) return launch(k_combine<T, true>);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kShifted) return p.k <= 2 ? launch(k_combine_odd<T, 2>) : launch(k_combine_odd<T, 4>);
+    return launch(k_combine<T, false>);
 }
 template <typename T, int GROUP, int FLIGHT>
 int combine_backward_as(const Rows &p) {
-    using A = Acc<T>;
-    const T *dy = (const T *)p.in, *rows = (const T *)p.rows;
-    const A *w = (const A *)p.weights;
     constexpr int threads = backward_threads(GROUP);
+    const RowMode mode = row_mode<T>(p.d, p.in, p.rows, p.out);
     const unsigned grid = token_blocks(p.tokens, threads / GROUP);
-    if (pieces_of_16<T>(p.d, p.in, p.rows, p.out))
-        k_combine_backward<T, GROUP, FLIGHT, true><<<grid, threads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
-    else
-        k_combine_backward<T, GROUP, FLIGHT, false><<<grid, threads, 0, p.s>>>(dy, rows, p.positions, w, p.tokens, p.k, p.d, (T *)p.out, (A *)p.dweights);
-    BGL_LAUNCH_CHECK();
-    return BGL_OK;
+    auto launch = [&](auto kernel) {
+        kernel<<<grid, threads, 0, p.s>>>((const T *)p.in, (const T *)p.rows, p.positions, (const Acc<T> *)p.weights, p.tokens,
+                                          p.k, p.d, (T *)p.out, (Acc<T> *)p.dweights);
+        BGL_LAUNCH_CHECK();
+        return (int)BGL_OK;
+    };
+    if (mode == kAligned) return launch(k_combine_backward<T, GROUP, FLIGHT, true>);
+    if (mode == kShifted) return launch(k_combine_backward_odd<T, GROUP>);
+    return launch(k_combine_backward<T, GROUP, FLIGHT, false>);
 }
 template <typename T>
 int combine_backward_as(const Rows &p) {
