@@ -393,9 +393,6 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
     const Columns<T, GROUP, MODE> c(mine, d);
     Pair<A> aw[kPieces][P::kPairs], ab[kPieces][P::kPairs];
     Pair<A> wv[MODE == kShifted ? 1 : kPieces][P::kPairs];
-    auto weight = [&](int i, int j) {
-        return MODE == kShifted ? weights[(i * P::kPairs + j) * kThreads + threadIdx.x] : wv[MODE == kShifted ? 0 : i][j];
-    };
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
@@ -408,6 +405,9 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
 #pragma unroll
             for (int j = 0; j < P::kPairs; ++j) weights[(i * P::kPairs + j) * kThreads + threadIdx.x] = wv[0][j];
     }
+    auto weight = [&](int i, int j) {
+        return MODE == kShifted ? weights[(i * P::kPairs + j) * kThreads + threadIdx.x] : wv[MODE == kShifted ? 0 : i][j];
+    };
     const A extra_w = w && c.has_extra() ? to_acc(w[c.extra]) : A(1);
     A extra_aw = 0, extra_ab = 0;
     // values to the next row to fetch, and to the row at hand
