@@ -34,15 +34,15 @@ int gmm_tensor_core(const void *a, const void *b, void *out, const GmmLayout &l,
                     int64_t d1, int64_t r, int64_t d2, int dtype, cudaStream_t s);
 
 // Gradients of the grouped product on the tensor cores (grouped_mm_grad_tc.cu).
-// Work comes in items: 256 x 256 tiles of da, and pieces of db's 256 x 256
-// tiles (a range of the segment's 64-row slices).
-constexpr int kGradSlice = 64, kGradTile = 256;
+// Work comes in items for pairs of CTAs: 512 x 256 tiles of da, and pieces of db's
+// 512 x 256 tiles (a range of the segment's 64-row slices).
+constexpr int kGradSlice = 64, kGradRows = 512, kGradCols = 256;
 
 // The schedule, written by one kernel into the caller's workspace.  Segments
 // are in the order of `order` in the arrays of db.
 struct GradLayout {
     int64_t *off;       // [r + 1] first row of each segment
-    int64_t *row_off;   // [r + 1] first 256-row tile of each segment (da)
+    int64_t *row_off;   // [r + 1] first 512-row tile of each segment (da)
     int32_t *order;     // [r] db's segments, long ones first
     int64_t *item_off;  // [r + 1] db's items before those of order[i]
     int64_t *cut_off;   // [r + 1] db's tiles of several pieces before those of order[i]
@@ -65,11 +65,12 @@ __host__ __device__ inline GradPieces grad_pieces(int64_t rows, int64_t most) {
 }
 
 struct GradTiles {
-    int64_t tiles1, tiles2;  // 256-column tiles of d1 and d2
-    int ctas;
+    int64_t cols;          // da: 256-column tiles of a row tile
+    int64_t tiles1, tiles2;  // db: tiles of a segment's block down and across
+    int pairs;
 };
 GradTiles gmm_grad_tiles(int64_t n, int64_t d1, int64_t r, int64_t d2);
-// At most this many partial tiles a CTA (k_grad_schedule's rule keeps to it).
+// At most this many partial tiles a pair (k_grad_schedule's rule keeps to it).
 constexpr int kGradSlots = 4;
 
 // da or db may be null (not wanted).

@@ -47,18 +47,18 @@ __device__ __forceinline__ Three block_scan(Three v, Three *warps, Three &total)
     return before;
 }
 
-// First row and first 256-row tile of each segment, and db's items; one block.
+// First row and first 512-row tile of each segment, and db's items; one block.
 // The rows are clamped as segment_mm's own schedule clamps them: negative
 // lengths count as 0 and no segment runs past n.
 //
-// Items are taken by whichever CTA is free, db's first and its long segments
-// first, da's small tiles last, so the CTAs end together.  A db tile is cut
-// into pieces where its sum is longer than half of a CTA's share of all work;
+// Items are taken by whichever pair of CTAs is free, db's first and its long segments
+// first, da's small tiles last, so the pairs end together.  A db tile is cut
+// into pieces where its sum is longer than half of a pair's share of all work;
 // that also bounds the partial tiles (a sum of L slices cut into pieces of P has
 // ceil(L / P) < 2 L / P of them where L > P, all sums together 2 * work / P <= 4 a
-// CTA).  A tile's read-out counts as kTileCost slices.  Measured with 500000 x 256
+// pair).  A tile's read-out counts as kTileCost slices.  Measured with 500000 x 256
 // x 256 over 64 segments (7,860 slices of db, 2,017 tiles of da): 240 us where
-// pieces could be as long as a CTA's share, 226 us so.
+// pieces could be as long as a pair's share, 226 us so.
 __global__ void __launch_bounds__(1024)
     k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, GradTiles t,
                     int64_t slices2, bool want_da, bool want_db, GradLayout l) {
@@ -75,13 +75,13 @@ __global__ void __launch_bounds__(1024)
         // to more than n, which no caller of a matching product gives, a second
         // scan counts them)
         Three total;
-        Three before = block_scan({len, (len + kGradTile - 1) / kGradTile, 0}, warps, total);
+        Three before = block_scan({len, (len + kGradRows - 1) / kGradRows, 0}, warps, total);
         int64_t first = rows + before.a, end = first + len;
         if (rows + total.a > n) {
             first = first < n ? first : n;
             end = end < n ? end : n;
             Three clamped;
-            before.b = block_scan({0, (end - first + kGradTile - 1) / kGradTile, 0}, warps, clamped).b;
+            before.b = block_scan({0, (end - first + kGradRows - 1) / kGradRows, 0}, warps, clamped).b;
             total.b = clamped.b;
         }
         int64_t mine = (end - first + kGradSlice - 1) / kGradSlice;
@@ -115,10 +115,10 @@ __global__ void __launch_bounds__(1024)
     }
     __syncthreads();
     const int64_t per_segment = t.tiles1 * t.tiles2;
-    const int64_t da_items = want_da ? tiles * t.tiles1 : 0;
+    const int64_t da_items = want_da ? tiles * t.cols : 0;
     const int64_t da_work = da_items * (slices2 + kTileCost);
     const int64_t db_work = slices * per_segment;
-    int64_t piece = (da_work + db_work + 2 * t.ctas - 1) / (2 * t.ctas);
+    int64_t piece = (da_work + db_work + 2 * t.pairs - 1) / (2 * t.pairs);
     if (piece < kShortest) piece = kShortest;
     int64_t items = 0, cut = 0, slots = 0;
     for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(1024)
         l.head[kHeadDbItems] = items;
         l.head[kHeadPiece] = piece;
         l.head[kHeadCut] = cut;
-        l.head[kHeadNext] = t.ctas;  // the first items are the CTAs' own numbers
+        l.head[kHeadNext] = t.pairs;  // the first items are the pairs' own numbers
     }
 }
 
@@ -361,9 +361,9 @@ GradLayout grad_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, i
     l.partial = nullptr;
     if (dtype == BGL_BF16) {
         // no tile is cut below 8 slices
-        int64_t slots = (int64_t)t.ctas * kGradSlots;
+        int64_t slots = (int64_t)t.pairs * kGradSlots;
         const int64_t most = t.tiles1 * t.tiles2 * 2 * (n / kGradSlice) / 8;
-        l.partial = c.take<float>((size_t)(slots < most ? slots : most) * kGradTile * kGradTile);
+        l.partial = c.take<float>((size_t)(slots < most ? slots : most) * kGradRows * kGradCols);
     }
     l.bytes = c.used + 256;
     return l;
