@@ -64,7 +64,7 @@ struct Item {
 };
 constexpr int kDa = 1, kDb = 2;
 constexpr size_t kSmem = 1024 + kStages * (size_t)kStageBytes + kEpiWarps * 4096 +
-                         8 * (2 * kStages + 2 * kQueue + 7) + kQueue * sizeof(Item) + 16;
+                         8 * (4 * kStages + 2 * kQueue + 5) + kQueue * sizeof(Item) + 16;
 
 // Last i in [0, n) with first[i] <= at, by the whole warp (33 ways a step).
 __device__ __forceinline__ int64_t warp_search(const int64_t *first, int64_t n, int64_t at) {
@@ -299,7 +299,10 @@ __device__ __forceinline__ Shape shape_of(const GradArgs &p, const Item &q, int 
     s.boxes_m = min(2 * s.halves, max(0, (m - s.first + 63) / 64));
     s.n = min(kGradCols, (n + 31) / 32 * 32);
     const int mine = s.n / 2, left = n - rank * mine;
-    s.boxes_n = min((mine + 63) / 64, max(0, (left + 63) / 64));
+    // the second CTA loads a box in any case (columns behind the operand's last, which
+    // no result comes from): the first does not run ahead of it in the ring
+    const int need = (left + 63) / 64, least = rank == 1 && s.boxes_m == 0;
+    s.boxes_n = min((mine + 63) / 64, max(least, need));
     s.slices = (k + kGradSlice - 1) / kGradSlice;
     return s;
 }
@@ -316,9 +319,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint4 *staging = reinterpret_cast<uint4 *>(ring + kStages * kStageBytes);
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + kStages * kStageBytes + kEpiWarps * 4096);
     uint64_t *empty = full + kStages;           // the MMAs have read the slice, in both CTAs
-    uint64_t *tail = empty + kStages;  // second CTA: the rows of a slice that is not whole are there
-    uint64_t *peer = tail + 1;         // first CTA: and end in zeros there
-    uint64_t *next_full = peer + 1;       // [kQueue] an item has been published
+    // Slices of db that are not whole, in turn (the ring holds at most kStages of them):
+    uint64_t *tail = empty + kStages;  // second CTA: the rows are there
+    uint64_t *peer = tail + kStages;   // first CTA: and end in zeros there
+    uint64_t *next_full = peer + kStages;       // [kQueue] an item has been published
     uint64_t *next_empty = next_full + kQueue;  // [kQueue] every role has read it
     uint64_t *acc_full = next_empty + kQueue;  // [2] a half of the accumulators is finished
     uint64_t *acc_empty = acc_full + 2;  // [2] first CTA: it has been read, in both CTAs
@@ -331,9 +335,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&tail[s], 1);
+            mbar_init(&peer[s], 1);
         }
-        mbar_init(tail, 1);
-        mbar_init(peer, 1);
         for (int s = 0; s < kQueue; ++s) {
             mbar_init(&next_full[s], 1);
             mbar_init(&next_empty[s], 2 + kEpiWarps + (rank == 0));
@@ -401,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp == kWarpLoad) {
         const uint32_t ring_at = in_cta(ring, rank);
-        int64_t it = 0;
+        int64_t it = 0, tails = 0;
         bool ok = true;
         Item q;
         for (int64_t t = 0; ok && take(t, q); ++t) {
@@ -427,8 +431,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (rank == 0) {
                         mbar_arrive_expect_tx(&full[s], k < whole ? both : mine);
                     } else if (k == whole) {
-                        bar = in_cta(tail, 1);
-                        mbar_arrive_expect_tx(tail, mine);
+                        uint64_t *at = &tail[tails++ % kStages];
+                        bar = in_cta(at, 1);
+                        mbar_arrive_expect_tx(at, mine);
                     }
                     const int32_t at = (da ? 0 : q.row0) + kGradSlice * k;
                     for (int b = 0; b < sh.boxes_m; ++b)
@@ -475,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             it += whole;
             if (ok && whole < sh.slices) {
                 const int s = (int)(it % kStages);
-                if (!(ok = warp_wait(rank ? tail : &full[s], (uint32_t)(rank ? tails : it / kStages) & 1, 3, abort))) break;
+                if (!(ok = warp_wait(rank ? &tail[tails % kStages] : &full[s], (uint32_t)((rank ? tails : it) / kStages) & 1, 3, abort))) break;
                 unsigned char *m = ring + s * kStageBytes;
                 const int rows = q.rows % kGradSlice, steps = (rows + 15) / 16;
                 const int zero = (steps * 16 - rows) * 8;  // 16-byte pieces of a box
@@ -487,9 +492,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (rank == 1) {
-                    if (lane == 0) arrive_in(peer, 0);
+                    if (lane == 0) arrive_in(&peer[tails % kStages], 0);
                 } else {
-                    if (!(ok = warp_wait(peer, (uint32_t)tails & 1, 9, abort))) break;
+                    if (!(ok = warp_wait(&peer[tails % kStages], (uint32_t)(tails / kStages) & 1, 9, abort))) break;
                     if (lane == 0) {
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         for (int h = 0; h < sh.halves; ++h)

@@ -86,6 +86,43 @@ def test_every_short_segment(dtype):
     check(randn(g, n, 64, dtype=dtype), randn(g, n, 128, dtype=dtype), randn(g, 141, 128, 64, dtype=dtype), seglen)
 
 
+@pytest.mark.parametrize("d1,d2", [(64, 72), (256, 256), (320, 8)])
+def test_sums_of_a_few_rows_one_after_another(d1, d2):
+    """Hundreds of sums of 1 to 130 rows a worker: several parts of a slice are under way at once."""
+    r = 6000
+    seglen = np.random.default_rng(31).integers(1, 131, r)
+    seglen[:5] = 1
+    seglen[-100:] = 3
+    n = int(seglen.sum())
+    g = gen(32)
+    grad, a, b = randn(g, n, d2, dtype=torch.bfloat16), randn(g, n, d1, dtype=torch.bfloat16), randn(g, r, d1, d2, dtype=torch.bfloat16)
+    none, db = ops.segment_mm_backward(grad, a, b, seglen, need_a=False)
+    assert none is None and _lib.lib().bgl_tc_error() == 0
+    da, none = ops.segment_mm_backward(grad, a, b, seglen, need_b=False)
+    assert none is None and _lib.lib().bgl_tc_error() == 0
+    both = ops.segment_mm_backward(grad, a, b, seglen)
+    assert _lib.lib().bgl_tc_error() == 0
+    assert torch.equal(da, both[0]) and torch.equal(db, both[1])
+    some = np.r_[0:40, r - 140:r - 80]  # these against float64
+    first = np.concatenate([[0], np.cumsum(seglen)])
+    at = torch.as_tensor(np.concatenate([np.arange(first[k], first[k + 1]) for k in some]), device="cuda")
+    ra, sa, rb, sb = reference(grad[at], a[at], b[torch.as_tensor(some, device="cuda")], seglen[some])
+    u, rnd = UNIT[torch.bfloat16], ROUND[torch.bfloat16]
+    assert bool(((da[at].double() - ra).abs() <= (d2 + 4) * u * sa + rnd * ra.abs()).all())
+    terms = torch.as_tensor(seglen[some], device="cuda").view(-1, 1, 1)
+    got = db[torch.as_tensor(some, device="cuda")].double()
+    assert bool(((got - rb).abs() <= (terms + 4) * u * sb + rnd * rb.abs()).all())
+
+
+@pytest.mark.parametrize("d1,d2", [(16, 8), (128, 16), (8, 264), (264, 8), (16, 2048)])
+def test_narrow_blocks_and_long_sums(d1, d2):
+    """Blocks that one of two workers has no values of, over hundreds of slices."""
+    seglen = np.array([20000, 0, 7001, 13])
+    n = int(seglen.sum())
+    g = gen(33)
+    check(randn(g, n, d2, dtype=torch.bfloat16), randn(g, n, d1, dtype=torch.bfloat16), randn(g, 4, d1, d2, dtype=torch.bfloat16), seglen)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_past_the_segments_and_empty_ones(dtype):
     g = gen(5)
