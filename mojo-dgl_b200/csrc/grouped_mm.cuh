@@ -71,7 +71,7 @@ struct GradTiles {
 };
 GradTiles gmm_grad_tiles(int64_t n, int64_t d1, int64_t r, int64_t d2);
 // At most this many partial tiles a pair (k_grad_schedule's rule keeps to it).
-constexpr int kGradSlots = 4;
+constexpr int kGradSlots = 3;
 
 // da or db may be null (not wanted).
 bool gmm_grad_tc_supported(const void *grad, const void *a, const void *b, const void *da,

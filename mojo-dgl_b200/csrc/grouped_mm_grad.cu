@@ -53,12 +53,14 @@ __device__ __forceinline__ Three block_scan(Three v, Three *warps, Three &total)
 //
 // Items are taken by whichever pair of CTAs is free, db's first and its long segments
 // first, da's small tiles last, so the pairs end together.  A db tile is cut
-// into pieces where its sum is longer than half of a pair's share of all work;
-// that also bounds the partial tiles (a sum of L slices cut into pieces of P has
-// ceil(L / P) < 2 L / P of them where L > P, all sums together 2 * work / P <= 4 a
-// pair).  A tile's read-out counts as kTileCost slices.  Measured with 500000 x 256
-// x 256 over 64 segments (7,860 slices of db, 2,017 tiles of da): 240 us where
-// pieces could be as long as a pair's share, 226 us so.
+// into pieces where its sum is longer than a pair's share of all work, or three
+// quarters of it where no tiles of da fill in behind; that also bounds the partial
+// tiles (a sum of L slices cut into pieces of P has ceil(L / P) < 2 L / P of them
+// where L > P, all sums together 2 * work / P < 3 a pair).  A tile's read-out counts
+// as kTileCost slices.  Measured with pieces up to half, three quarters and the whole
+// of the share: 500000 x 256 x 256 over 64 segments 224, 222, 210 us; 300000 x 256 x
+// 128 over 5: 204, 160, 144; db alone, 500000 x 256 x 256: 142, 132, 149, and 32768 x
+// 2048 x 1024 over 16 uneven ones: 189, 152, 148.
 __global__ void __launch_bounds__(1024)
     k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, GradTiles t,
                     int64_t slices2, bool want_da, bool want_db, GradLayout l) {
@@ -118,7 +120,8 @@ __global__ void __launch_bounds__(1024)
     const int64_t da_items = want_da ? tiles * t.cols : 0;
     const int64_t da_work = da_items * (slices2 + kTileCost);
     const int64_t db_work = slices * per_segment;
-    int64_t piece = (da_work + db_work + 2 * t.pairs - 1) / (2 * t.pairs);
+    const int64_t quarters = (want_da ? 4 : 3) * (da_work + db_work);
+    int64_t piece = (quarters + 4 * t.pairs - 1) / (4 * t.pairs);
     if (piece < kShortest) piece = kShortest;
     int64_t items = 0, cut = 0, slots = 0;
     for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {
