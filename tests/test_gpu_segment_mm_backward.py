@@ -123,6 +123,18 @@ def test_narrow_blocks_and_long_sums(d1, d2):
     check(randn(g, n, d2, dtype=torch.bfloat16), randn(g, n, d1, dtype=torch.bfloat16), randn(g, 4, d1, d2, dtype=torch.bfloat16), seglen)
 
 
+@pytest.mark.parametrize("n,r,d1,d2", [(70000, 9, 256, 256), (70001, 300, 200, 256), (141000, 64, 72, 128), (66001, 1, 8, 256), (300007, 1200, 256, 64)])
+def test_blocks_of_one_tile_and_many_rows(n, r, d1, d2):
+    """Segments end everywhere in a tile, the last rows belong to none."""
+    g = gen(34 + d1)
+    seglen = lengths(n, n - 37, r, zero=(r // 3,) if r > 1 else ())
+    grad, a, b = randn(g, n, d2, dtype=torch.bfloat16), randn(g, n, d1, dtype=torch.bfloat16), randn(g, r, d1, d2, dtype=torch.bfloat16)
+    first = check(grad, a, b, seglen)
+    assert not first[0][-37:].any()
+    again = ops.segment_mm_backward(grad, a, b, seglen)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_past_the_segments_and_empty_ones(dtype):
     g = gen(5)
