@@ -13,6 +13,7 @@
 // Memory bounds the three of them: each reads a token's row once for its k
 // choices, in 16-byte pieces where the row length and the addresses allow, the
 // lanes of a token side by side over its row.
+#include "after.cuh"
 #include "rows.cuh"
 
 namespace bgl {
@@ -56,6 +57,7 @@ Plan plan_of(int64_t items, int64_t experts) {
 __global__ void __launch_bounds__(kThreads)
     k_plan_count(const Plan p, const int64_t *__restrict__ indices, int32_t *__restrict__ chunk_bins) {
     extern __shared__ int32_t bins[];
+    next_may_start();
     for (int b = threadIdx.x; b <= p.experts; b += blockDim.x) bins[b] = 0;
     __syncthreads();
     const int64_t per = p.per_warp * p.warps, i0 = blockIdx.x * per;
@@ -72,6 +74,8 @@ __global__ void __launch_bounds__(kThreads)
     k_plan_scan(const Plan p, int32_t *__restrict__ chunk_bins, int32_t *__restrict__ totals,
                 int64_t *__restrict__ counts) {
     const int lane = threadIdx.x & 31, bin = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    next_may_start();
+    before_is_done();
     if (bin > p.experts) return;
     int32_t sum = 0;
     for (int64_t c0 = 0; c0 < p.chunks; c0 += 32) {
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(kThreads)
 // Rows of a chunk's items.  With one chunk, its own counts are the totals.
 __global__ void __launch_bounds__(kThreads)
     k_plan_place(const Plan p, const int64_t *__restrict__ indices,
-                 const int32_t *__restrict__ chunk_bins, const int32_t *__restrict__ totals,
+                 const int32_t *chunk_bins, const int32_t *totals,
                  int32_t *__restrict__ positions, int64_t *__restrict__ counts) {
     extern __shared__ int32_t next[];  // [warp][bin]
     __shared__ int32_t warp_sums[32];
@@ -108,6 +112,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll 4
     for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[bin_of(indices[i], p.experts)], 1);
     __syncthreads();
+    before_is_done();  // up to here the kernel needs no other's results
     // each bin's first row: all items of lower bins, those of its own in earlier
     // chunks, those of this chunk's earlier warps
     int32_t before = 0;
@@ -639,12 +644,14 @@ int bgl_expert_plan(const int64_t *indices, int64_t items, int64_t experts, int6
         totals = c.take<int32_t>((size_t)experts + 1);
         k_plan_count<<<(unsigned)p.chunks, kThreads, (experts + 1) * sizeof(int32_t), s>>>(p, indices, chunk_bins);
         BGL_LAUNCH_CHECK();
-        k_plan_scan<<<(unsigned)((experts + 8) / 8), kThreads, 0, s>>>(p, chunk_bins, totals, counts);
-        BGL_LAUNCH_CHECK();
+        BGL_CUDA(launch_after(k_plan_scan, (unsigned)((experts + 8) / 8), kThreads, 0, s, p, chunk_bins, totals, counts));
     }
-    k_plan_place<<<(unsigned)(p.chunks > 0 ? p.chunks : 1), p.warps * 32,
-                   p.warps * (experts + 1) * sizeof(int32_t), s>>>(p, indices, chunk_bins, totals,
-                                                                   positions, counts);
+    const unsigned chunks = (unsigned)(p.chunks > 0 ? p.chunks : 1), threads = p.warps * 32;
+    const size_t smem = p.warps * (experts + 1) * sizeof(int32_t);
+    if (p.chunks > 1)
+        BGL_CUDA(launch_after(k_plan_place, chunks, threads, smem, s, p, indices, chunk_bins, totals, positions, counts));
+    else
+        k_plan_place<<<chunks, threads, smem, s>>>(p, indices, chunk_bins, totals, positions, counts);
     BGL_LAUNCH_CHECK();
     return BGL_OK;
 }

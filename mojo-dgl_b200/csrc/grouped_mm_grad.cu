@@ -4,6 +4,7 @@
 //   da[i] = dout[i] @ b[r(i)]^T        db[r] = a[rows of r]^T @ dout[rows of r]
 //
 // Rows past the last segment have da = 0; a segment without rows has db = 0.
+#include "after.cuh"
 #include "grouped_mm.cuh"
 #include "rows.cuh"
 
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(1024)
     constexpr int kSorted = 256;  // more segments than this stay in order
     __shared__ Three warps[32];
     __shared__ int64_t lens[kSorted];
+    next_may_start();
     int64_t rows = 0, tiles = 0, slices = 0;
     for (int64_t i0 = 0; i0 < r; i0 += blockDim.x) {
         const int64_t i = i0 + threadIdx.x;

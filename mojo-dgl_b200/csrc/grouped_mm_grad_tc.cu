@@ -30,6 +30,7 @@
 // tiles, which k_grad_finish adds in order: the same bits on every run.
 //
 // Every mbarrier wait is bounded, with the abort protocol of grouped_mm_tc.cu.
+#include "after.cuh"
 #include "grouped_mm.cuh"
 #include "tcgen05.cuh"
 
@@ -361,6 +362,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     cluster_barrier();  // the other CTA's barriers are initialised
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    next_may_start();
+    before_is_done();
 
     // Item t of this CTA, for a whole warp: false when none is left.
     auto take = [&](int64_t t, Item &q) {
@@ -620,6 +623,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Adds the pieces of db's cut tiles, 16 columns a thread, and zeroes the rows of
 // da past the last segment.
 __global__ void __launch_bounds__(256) k_grad_finish(const GradArgs args) {
+    before_is_done();
     if (args.da) {
         const int64_t first = args.off[args.r] * args.d1 / 8, end = args.n * args.d1 / 8;
         const int64_t block = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
@@ -754,10 +758,8 @@ int gmm_grad_tensor_core(const void *grad, const void *a, const void *b, void *d
     args.d1 = (int32_t)d1;
     args.d2 = (int32_t)d2;
     BGL_CUDA(cudaFuncSetAttribute(k_grad_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-    k_grad_tc<<<2 * t.pairs, kThreads, kSmem, s>>>(map_a, map_g, map_b, map_da, map_db, args);
-    BGL_LAUNCH_CHECK();
-    k_grad_finish<<<dim3((unsigned)t.pairs, 32), 256, 0, s>>>(args);
-    BGL_LAUNCH_CHECK();
+    BGL_CUDA(launch_after(k_grad_tc, 2 * t.pairs, kThreads, kSmem, s, map_a, map_g, map_b, map_da, map_db, args));
+    BGL_CUDA(launch_after(k_grad_finish, dim3((unsigned)t.pairs, 32), 256, 0, s, args));
     return BGL_OK;
 }
 

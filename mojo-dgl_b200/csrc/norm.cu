@@ -17,6 +17,7 @@
 // k_layer_norm_join adds in order: the same bits on every run.
 //
 // Rows longer than kMostHeld go through loops that read them again (from L2).
+#include "after.cuh"
 #include "rows.cuh"
 
 namespace bgl {
@@ -385,6 +386,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), backward_resident(GROUP, N,
     Pair<A> *weights = reinterpret_cast<Pair<A> *>(raw);      // kShifted: [piece][pair][thread]
     A *columns = reinterpret_cast<A *>(raw + kWeights);       // [d], after the rows
     uint4 *ring = reinterpret_cast<uint4 *>(raw + kWeights);  // [stage][x, dy][piece][thread]
+    next_may_start();
     int turn = 0;
     const int64_t run = blockIdx.x / kShare, runs = gridDim.x / kShare;
     const int64_t begin = rows * run / runs, end = rows * (run + 1) / runs;
@@ -638,10 +640,11 @@ __global__ void __launch_bounds__(kThreads)
 // order.  blockIdx.y: 0 dw, 1 db.
 template <typename A, typename W>
 __global__ void __launch_bounds__(1024)
-    k_layer_norm_join(const A *__restrict__ partial, int64_t parts, int64_t d, W *__restrict__ dw,
+    k_layer_norm_join(const A *partial, int64_t parts, int64_t d, W *__restrict__ dw,
                       W *__restrict__ db) {
     __shared__ A sums[32][33];
     W *out = blockIdx.y ? db : dw;
+    before_is_done();
     if (!out) return;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t col = (int64_t)blockIdx.x * 32 + tx;
@@ -828,9 +831,8 @@ int backward(const Backward &p) {
         if (rc) return rc;
     }
     if (sums) {
-        k_layer_norm_join<A, W><<<dim3((unsigned)((p.d + 31) / 32), 2), 1024, 0, p.s>>>(
-            partial, parts, p.d, (W *)p.dw, (W *)p.db);
-        BGL_LAUNCH_CHECK();
+        BGL_CUDA(launch_after(k_layer_norm_join<A, W>, dim3((unsigned)((p.d + 31) / 32), 2), 1024, 0, p.s,
+                              partial, parts, p.d, (W *)p.dw, (W *)p.db));
     }
     return BGL_OK;
 }
