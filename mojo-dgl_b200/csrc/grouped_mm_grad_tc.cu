@@ -12,7 +12,11 @@
 // K slice of 64 brings 32 KB + 16 KB to a CTA for 2 x 4 MMAs of 256 x 256 x 16, where
 // a 256 x 256 tile of its own takes 64 KB: three quarters of the traffic from L2, and
 // four slices in the ring instead of three.  32768 x 2048 x 1024 over 16 segments: 285
-// us with a tile a CTA, 278 so; 500000 x 256 x 256 over 64: 228 and 222.
+// us with a tile a CTA, 278 so; 500000 x 256 x 256 over 64: 228 and 222 (now 270 and
+// 204).  The wide one waits for tiles for 23 % of the time and runs into the power
+// limit; the narrow one is bound by memory (984 MB in 166 us in the kernel).  Taking
+// da's tiles along with db's sums, 256 rows at a time, so that grad would be read from
+// DRAM once, took 202 us in the kernel: the loads under way are then half L2's.
 //
 // One persistent launch holds both products.  Warp 10 of a pair's first CTA takes
 // the next item (an atomic counter; which pair does what does not change any
@@ -179,15 +183,20 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// A waiting thread may sleep that long at a time (it wakes up when the phase is over):
+// polling took a quarter of the issue slots, and power (276 -> 270 us where the power
+// limit holds, 209 -> 204 for the narrow case).
+constexpr uint32_t kSleepNs = 20000;
+
 // The bounded wait for what the other CTA of the pair may have written or arrived on.
 __device__ __forceinline__ bool pair_try_wait(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.b32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(kSleepNs)
         : "memory");
     return ok != 0;
 }
