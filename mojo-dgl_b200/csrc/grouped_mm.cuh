@@ -38,6 +38,8 @@ int gmm_tensor_core(const void *a, const void *b, void *out, const GmmLayout &l,
 // 512 x 256 tiles (a range of the segment's 64-row slices).
 constexpr int kGradSlice = 64, kGradRows = 512, kGradCols = 256;
 
+constexpr int kGradShortest = 8;  // slices; a sum of so many is not cut
+
 // The schedule, written by one kernel into the caller's workspace.  Segments
 // are in the order of `order` in the arrays of db.
 struct GradLayout {

@@ -65,7 +65,7 @@ __device__ __forceinline__ Three block_scan(Three v, Three *warps, Three &total)
 __global__ void __launch_bounds__(1024)
     k_grad_schedule(const int64_t *__restrict__ seglen, int64_t r, int64_t n, GradTiles t,
                     int64_t slices2, bool want_da, bool want_db, GradLayout l) {
-    constexpr int64_t kTileCost = 2, kShortest = 8;
+    constexpr int64_t kTileCost = 2;
     constexpr int kSorted = 256;  // more segments than this stay in order
     __shared__ Three warps[32];
     __shared__ int64_t lens[kSorted];
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(1024)
     const int64_t db_work = slices * per_segment;
     const int64_t quarters = (want_da ? 4 : 3) * (da_work + db_work);
     int64_t piece = (quarters + 4 * t.pairs - 1) / (4 * t.pairs);
-    if (piece < kShortest) piece = kShortest;
+    if (piece < kGradShortest) piece = kGradShortest;
     int64_t items = 0, cut = 0, slots = 0;
     for (int64_t k0 = 0; want_db && k0 < r; k0 += blockDim.x) {
         const int64_t k = k0 + threadIdx.x;
@@ -365,9 +365,9 @@ GradLayout grad_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, i
     l.head = c.take<int64_t>(kHead);
     l.partial = nullptr;
     if (dtype == BGL_BF16) {
-        // no tile is cut below 8 slices
+        // no tile is cut below kGradShortest slices
         int64_t slots = (int64_t)t.pairs * kGradSlots;
-        const int64_t most = t.tiles1 * t.tiles2 * 2 * (n / kGradSlice) / 8;
+        const int64_t most = t.tiles1 * t.tiles2 * 2 * (n / kGradSlice) / kGradShortest;
         l.partial = c.take<float>((size_t)(slots < most ? slots : most) * kGradRows * kGradCols);
     }
     l.bytes = c.used + 256;
