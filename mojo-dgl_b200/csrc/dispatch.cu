@@ -20,8 +20,8 @@ namespace bgl {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxBins = 8192;           // experts + 1: shared-memory counters
-constexpr int kCounters = 48 * 1024 / 4; // of a block
+constexpr int kMaxBins = 8192;  // experts + 1: shared-memory counters
+constexpr int kCounters = 48 * 1024 / 4 - 32;  // of a block: 48 KB, less the sums of its warps
 constexpr int kMaxChunks = 1024;
 
 // ---------------------------------------------------------------- the plan
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads)
     k_plan_place(const Plan p, const int64_t *__restrict__ indices,
                  const int32_t *chunk_bins, const int32_t *totals,
                  int32_t *__restrict__ positions, int64_t *__restrict__ counts) {
-    extern __shared__ int32_t next[];  // [warp][bin]
+    extern __shared__ int32_t next[];   // [warp][bin], at most kCounters
     __shared__ int32_t warp_sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = p.experts + 1;
     for (int b = threadIdx.x; b < p.warps * bins; b += blockDim.x) next[b] = 0;
