@@ -17,9 +17,16 @@ namespace bgl {
 int fail(int code, const char *fmt, ...);
 void clear_error();
 
+// A failed call fails alone: the runtime's record of it is cleared, or the next
+// launch check would report it for another call.
+inline cudaError_t cleared(cudaError_t e) {
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e;
+}
+
 #define BGL_CUDA(call)                                                                   \
     do {                                                                                 \
-        cudaError_t e_ = (call);                                                         \
+        cudaError_t e_ = ::bgl::cleared(call);                                           \
         if (e_ != cudaSuccess)                                                           \
             return ::bgl::fail(BGL_E_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_)); \
     } while (0)

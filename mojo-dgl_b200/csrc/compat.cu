@@ -21,7 +21,7 @@ struct DevBuf {
     void *p = nullptr;
     cudaError_t err = cudaSuccess;
     explicit DevBuf(size_t bytes) {
-        if (bytes) err = cudaMalloc(&p, bytes);
+        if (bytes) err = cleared(cudaMalloc(&p, bytes));
     }
     ~DevBuf() {
         if (p) cudaFree(p);

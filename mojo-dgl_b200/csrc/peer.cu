@@ -87,7 +87,7 @@ int bgl_ipc_open(const void *handle, int64_t offset, int64_t bytes, void **ptr) 
         rc = fail(BGL_E_INVALID, "bgl_ipc_open: %lld bytes at offset %lld leave the %zu-byte "
                   "exported allocation", (long long)bytes, (long long)offset, size);
     if (rc != BGL_OK) {
-        cudaIpcCloseMemHandle(base);
+        (void)cleared(cudaIpcCloseMemHandle(base));
         return rc;
     }
     *ptr = static_cast<unsigned char *>(base) + offset;

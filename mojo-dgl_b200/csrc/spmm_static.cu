@@ -113,7 +113,7 @@ int scratch_address(void **out) {
     // Not resolved in this context yet (or no context is current, in which
     // case the runtime binds the device's primary context here).
     void *p = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&p, g_spmm_scratch);
+    cudaError_t e = cleared(cudaGetSymbolAddress(&p, g_spmm_scratch));
     if (e != cudaSuccess || p == nullptr)
         return fail(BGL_E_CUDA, "cudaGetSymbolAddress(static gspmm scratch) failed: %s",
                     cudaGetErrorString(e));

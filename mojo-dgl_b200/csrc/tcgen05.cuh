@@ -20,7 +20,7 @@ cudaError_t take_tc_error(int *code) {
     const int zero = 0;
     cudaError_t e = cudaMemcpyFromSymbol(code, g_tc_error, sizeof(int));
     if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(int));
-    return e;
+    return cleared(e);
 }
 
 constexpr unsigned long long kTimeoutNs = 2000000000ull;  // 2 s per wait
