@@ -289,7 +289,8 @@ int bgl_layer_norm_backward(const void *grad, const void *x, const void *mean, c
  * the remaining places.  NaN ranks first, and makes the weights that depend on
  * it NaN.  Limits: 1,024 experts, k <= 32, 32 groups.
  * The backward call gives dlogits (logits' dtype) of the weights at the given
- * indices; an index outside [0, experts) has no gradient. */
+ * indices; an index outside [0, experts) has no gradient, nor has an expert
+ * whose logit is -inf (weights over nothing but such ones: all zeros). */
 int bgl_route_topk(const void *logits, const float *bias, int64_t tokens, int64_t experts,
                    int64_t k, int score, int64_t num_groups, int64_t topk_groups, int group_top,
                    int renormalize, double scale, float *weights, int64_t *indices, int dtype,

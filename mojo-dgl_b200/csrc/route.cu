@@ -462,6 +462,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_route_topk_backward(const Route
         }
         if (!dense) {
             if (!a.sigmoid) most = lanes_max<LANES>(most);
+            if (most == -INFINITY) most = 0;  // chosen elsewhere, all of them masked: no gradient
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const float logit = s[i];

@@ -104,7 +104,8 @@ def route_topk_backward(grad, logits, indices, *, score="softmax", renormalize=T
     ``grad`` is the gradient of the weights, (tokens, k), ``indices`` the
     chosen experts; the other arguments are the forward call's.  The choice
     itself, and so the bias, has no gradient.  Places with index -1 (any index
-    that is not an expert's) have none either.  Returns (tokens, experts) in the
+    that is not an expert's) have none either, nor have masked experts (logits of
+    -inf) that a choice made elsewhere holds.  Returns (tokens, experts) in the
     logits' type.
     """
     kind, (grad, logits, indices) = T.operands(grad, logits, indices)
