@@ -91,8 +91,8 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&v)[4]) {
     *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(o);
 }
 
-// A sum of weights to divide by: the smallest normal number where all of them
-// underflowed (their quotients are then 0), NaN where one of them is NaN.
+// A sum of weights to divide by: the smallest normal number where there are none
+// (their quotients are then 0), NaN where one of them is NaN.
 __device__ __forceinline__ float at_least_tiny(float sum) {
     return sum < 1.17549435e-38f ? 1.17549435e-38f : sum;
 }
@@ -119,6 +119,27 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
+}
+
+// The k weights of a token whose sigmoids add up to less than kFar (`far`; the warp's
+// other tokens take part).  From -88.7 on they underflow, but their shares in the sum do
+// not: 1 + exp(x) is 1 there, and the sigmoids are the exponentials, which are taken
+// relative to the best one's.  Apart from the kernel, so that the way past it is short
+// (65536 x 256 in groups: 51.3 us without it, 52.3 so, 53.5 with a branch for each token).
+constexpr float kFar = 1e-9f;
+template <typename T>
+__device__ __noinline__ void far_weights(const T *x, const int *pick, int k, float scale, bool far, float *weights) {
+    const int own = threadIdx.x & (kLanes - 1);
+    float most = -INFINITY, total = 0;
+    for (int j = own; j < k; j += kLanes)
+        if (pick[j] >= 0) most = fmaxf(most, to_acc(x[pick[j]]));
+    most = lanes_max<kLanes>(most);
+    for (int j = own; j < k; j += kLanes)
+        if (pick[j] >= 0) total += expf(to_acc(x[pick[j]]) - most);
+    total = lanes_sum<kLanes>(total);
+    if (!far) return;
+    for (int j = own; j < k; j += kLanes)
+        if (pick[j] >= 0) weights[j] = expf(to_acc(x[pick[j]]) - most) / total * scale;
 }
 
 // A token's scores in shared memory: kLanes runs of subs * 8, 4 apart.
@@ -405,6 +426,10 @@ __global__ void __launch_bounds__(kSelect, SUBS > 4 ? 1 : 18) k_route_topk(const
             a.weights[t * a.k + j] = e >= 0 ? w[i] * a.scale : 0.0f;
             a.indices[t * a.k + j] = e;
         }
+        if (a.renormalize && a.sigmoid) {
+            const bool far = total < kFar && pick[0] >= 0;
+            if (__any_sync(0xffffffffu, far)) far_weights(x, pick, a.k, a.scale, far && live, a.weights + t * a.k);
+        }
         __syncwarp();
     }
 }
@@ -461,8 +486,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_route_topk_backward(const Route
             most = fmaxf(most, s[i]);
         }
         if (!dense) {
-            if (!a.sigmoid) most = lanes_max<LANES>(most);
-            if (most == -INFINITY) most = 0;  // chosen elsewhere, all of them masked: no gradient
+            if (!a.sigmoid) {
+                most = lanes_max<LANES>(most);
+                if (most == -INFINITY) most = 0;  // chosen elsewhere, all of them masked: no gradient
+            }
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const float logit = s[i];
@@ -474,7 +501,23 @@ __global__ void __launch_bounds__(kWarps * 32) k_route_topk_backward(const Route
                 if (a.sigmoid && at[i] >= 0 && a.renormalize) s[i] *= sigmoid_of(-logit);
             }
             if (a.renormalize) {
-                total = at_least_tiny(lanes_sum<LANES>(total));
+                total = lanes_sum<LANES>(total);
+                if (a.sigmoid && __any_sync(0xffffffffu, total < kFar && most > -INFINITY)) {
+                    // as far_weights: by the exponentials, whose slope's other factor is 1
+                    const bool far = total < kFar;
+                    most = lanes_max<LANES>(most);
+                    float far_total = 0, far_dot = 0;
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        if (!far || at[i] < 0) continue;
+                        s[i] = most > -INFINITY ? expf(to_acc(x[at[i]]) - most) : 0.0f;
+                        far_total += s[i];
+                        far_dot += s[i] * g[i];
+                    }
+                    far_total = lanes_sum<LANES>(far_total);
+                    if (far) total = far_total, dot = far_dot;
+                }
+                total = at_least_tiny(total);
                 dot = lanes_sum<LANES>(dot) / total;
 #pragma unroll
                 for (int i = 0; i < kEach; ++i)
