@@ -265,7 +265,7 @@ int bgl_tc_error(void);
  * Layer norm over the last axis of x (rows, d):
  *   y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias
  * weight and bias (d values) may be NULL, as may the outputs mean and rstd
- * (rows values each).  wdtype is dtype, or BGL_F32 for bf16 rows; mean and rstd
+ * (rows values each); y must not be x.  wdtype is dtype, or BGL_F32 for bf16 rows; mean and rstd
  * are float32, float64 for BGL_F64.  The backward call takes the mean and rstd
  * of the forward one; dx, dweight, dbias may be NULL (not computed), dweight and
  * dbias have wdtype.  The sums over rows have a fixed order. */

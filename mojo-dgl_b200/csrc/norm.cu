@@ -11,6 +11,14 @@
 // of the centred values in registers, not a difference of sums.  Groups walk over
 // rows with the next row's loads in flight while this one is reduced and written.
 //
+// A mean is off by a few units in its last place.  Where that shows (kFar), what the
+// centred values add up to says by how much, and they are centred again: a row of equal
+// values gave y up to 4 times w without it.  That is left for the end, where the rows
+// that need it are read again (8192 x 4096 bf16: 35 us a call without such rows, 61 with
+// one, 136 with all).  Doing it for every row, in the reduction of the squares, took 33.3
+// -> 36.6 us; asking each row whether it needs it 31.6 -> 31.8 in the kernel (65536 x 509:
+// 29.5 -> 31.5, 16384 x 2047 float32, which spilled before: 54.9 -> 47.4).
+//
 // Backward, the thread that holds a column of this row holds it of every row it
 // walks over, so dw and db add up in registers beside dx and x and dy are read
 // once for all three.  At the end a block leaves one partial row of each, which
@@ -156,6 +164,76 @@ __device__ __forceinline__ void group_sums(A (&v)[K], A (*smem)[K * (threads_of(
     }
 }
 
+// The same over one of the block's groups alone; what its threads wrote before comes
+// before what they write after.
+template <int GROUP, typename A>
+__device__ __forceinline__ A lone_sum(A v, A (*smem)[threads_of(GROUP) / 32], int &turn) {
+    constexpr int kLanes = GROUP < 32 ? GROUP : 32;
+    const unsigned lanes = (0xffffffffu >> (32 - kLanes)) << (threadIdx.x & 31 & ~(kLanes - 1));
+    __syncwarp(lanes);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(lanes, v, o);
+    if constexpr (GROUP > 32) {
+        const int group = threadIdx.x / GROUP;
+        if ((threadIdx.x & 31) == 0) smem[turn][threadIdx.x >> 5] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(GROUP) : "memory");
+        v = 0;
+        for (int i = 0; i < GROUP / 32; ++i) v += smem[turn][group * (GROUP / 32) + i];
+        turn ^= 1;
+    }
+    return v;
+}
+
+// f(column, value) over the thread's columns of a row, four loads at a time.
+template <int GROUP, typename T, typename F>
+__device__ __forceinline__ void walk(const T *row, int t, int d, F &&f) {
+#pragma unroll 1
+    for (int i = t; i < d; i += 4 * GROUP) {
+        T v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * GROUP < d) v[j] = row[i + j * GROUP];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * GROUP < d) f(i + j * GROUP, to_acc(v[j]));
+    }
+}
+
+// Centres rows whose mean is more than kFar + 1 times their spread a second time: a
+// group's own rows, from memory, once it has written all of them.  (It looks at them
+// where one passes kFar, so what becomes of a row does not depend on the others.)
+constexpr int kFar = 16;
+template <int GROUP, typename T, typename W>
+__device__ __forceinline__ void recentre(const T *x, const W *w, const W *b, int64_t row, int64_t rows, int64_t stride,
+                                         int64_t d, Acc<T> eps, T *y, Acc<T> *mean, Acc<T> *rstd,
+                                         Acc<T> (*smem)[threads_of(GROUP) / 32], int turn) {
+    using A = Acc<T>;
+    const int t = threadIdx.x % GROUP, n = (int)d;
+    for (; row < rows; row += stride) {
+        const T *from = x + row * d;
+        A s = 0, q = 0, e = 0;
+        walk<GROUP>(from, t, n, [&](int, A v) { s += v; });
+        const A mu = lone_sum<GROUP>(s, smem, turn) / A(d);
+        walk<GROUP>(from, t, n, [&](int, A v) { v -= mu, q += v * v, e += v; });
+        q = lone_sum<GROUP>(q, smem, turn) / A(d);
+        const A off = lone_sum<GROUP>(e, smem, turn) / A(d);
+        if (!(fabs(mu) > A(kFar + 1) * sqrt(q + eps))) continue;
+        q = 0;
+        walk<GROUP>(from, t, n, [&](int, A v) { v = v - mu - off, q += v * v; });
+        const A rs = A(1) / sqrt(lone_sum<GROUP>(q, smem, turn) / A(d) + eps);
+        walk<GROUP>(from, t, n, [&](int i, A v) {
+            v = (v - mu - off) * rs;
+            if (w) v *= to_acc(w[i]);
+            if (b) v += to_acc(b[i]);
+            y[row * d + i] = from_acc<T>(v);
+        });
+        if (t == 0) {
+            if (mean) mean[row] = mu + off;
+            if (rstd) rstd[row] = rs;
+        }
+    }
+}
+
 // Blocks an SM that the forward pass is compiled for, and the grid filled with.
 __host__ __device__ constexpr int forward_resident(int group, int values, int size) {
     return (size == 8 ? 3 : values == 8 ? 5 : 4) * kThreads / threads_of(group);
@@ -266,6 +344,7 @@ __global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, 
     };
     fetch(row);
     // whole groups take part in the block's barriers even behind the last row
+    bool far = false;
     for (int64_t r0 = first; r0 < rows; r0 += stride, row += stride) {
         const bool live = row < rows;
         Pair<A> v[kPieces][P::kPairs];
@@ -327,7 +406,9 @@ __global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, 
             if (mean) mean[row] = mu;
             if (rstd) rstd[row] = rs;
         }
+        far |= fabs(mu) * rs > A(kFar);
     }
+    if (far) recentre<GROUP>(x, w, b, first + threadIdx.x / GROUP, rows, stride, d, eps, y, mean, rstd, smem, turn);
 }
 
 // Blocks an SM that the backward pass is compiled for: what its registers allow
@@ -559,20 +640,29 @@ __global__ void __launch_bounds__(kThreads)
         A s = 0;
         for (int64_t i = threadIdx.x; i < d; i += blockDim.x) s += to_acc(xr[i]);
         const A mu = block_sum(s, smem) / A(d);
-        s = 0;
-        for (int64_t i = threadIdx.x; i < d; i += blockDim.x) {
-            const A c = to_acc(xr[i]) - mu;
-            s += c * c;
+        auto spread = [&](A off) {
+            s = 0;
+            for (int64_t i = threadIdx.x; i < d; i += blockDim.x) {
+                const A c = to_acc(xr[i]) - mu - off;
+                s += c * c;
+            }
+            return A(1) / sqrt(block_sum(s, smem) / A(d) + eps);
+        };
+        A off = 0, rs = spread(off);
+        if (fabs(mu) * rs > A(kFar)) {
+            s = 0;
+            for (int64_t i = threadIdx.x; i < d; i += blockDim.x) s += to_acc(xr[i]) - mu;
+            off = block_sum(s, smem) / A(d);
+            rs = spread(off);
         }
-        const A rs = A(1) / sqrt(block_sum(s, smem) / A(d) + eps);
         for (int64_t i = threadIdx.x; i < d; i += blockDim.x) {
-            A v = (to_acc(xr[i]) - mu) * rs;
+            A v = (to_acc(xr[i]) - mu - off) * rs;
             if (w) v *= to_acc(w[i]);
             if (b) v += to_acc(b[i]);
             y[row * d + i] = from_acc<T>(v);
         }
         if (threadIdx.x == 0) {
-            if (mean) mean[row] = mu;
+            if (mean) mean[row] = mu + off;
             if (rstd) rstd[row] = rs;
         }
     }
