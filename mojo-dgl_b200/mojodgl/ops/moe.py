@@ -180,6 +180,20 @@ def _positions(positions):
     return shape
 
 
+def _places(dev, positions):
+    """The positions as int32 on the device; those beyond its range at its ends,
+    which lie outside all rows (a cast alone would take their low halves)."""
+    if positions.dtype is torch.int32:
+        return T.on(dev, positions, torch.int32)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    if T.is_torch(positions):
+        positions = positions.to(torch.int64).clamp(low, high)
+    elif positions.dtype != np.int32:
+        span = np.iinfo(positions.dtype)
+        positions = positions.clip(max(low, span.min), min(high, span.max)).astype(np.int32)
+    return T.on(dev, positions, torch.int32)
+
+
 def _matrix(x, what, rows):
     shape = x.shape
     if len(shape) != 2 or shape[0] != rows:
@@ -208,7 +222,7 @@ def dispatch(x, positions):
     d = _matrix(x, "x", tokens)
     dtype = T.float_type(x)
     dev = T.device()
-    xt, pt = T.on(dev, x, dtype), T.on(dev, positions, torch.int32)
+    xt, pt = T.on(dev, x, dtype), _places(dev, positions)
     rows = xt.new_empty(tokens * k, d)
     check(lib().bgl_dispatch_rows(T.address(xt), T.address(pt), tokens, k, d, T.address(rows),
                                   T.code_of(dtype), T.stream()), "dispatch")
@@ -229,7 +243,7 @@ def combine(rows, positions, weights=None):
     _weights(weights, tokens, k)
     dtype = T.float_type(rows)
     dev = T.device()
-    rt, pt = T.on(dev, rows, dtype), T.on(dev, positions, torch.int32)
+    rt, pt = T.on(dev, rows, dtype), _places(dev, positions)
     wt = T.on(dev, weights, _weight_type(dtype))
     y = rt.new_empty(tokens, d)
     check(lib().bgl_combine_rows(T.address(rt), T.address(pt), T.address(wt), tokens, k, d, T.address(y),
@@ -253,7 +267,7 @@ def combine_backward(grad, rows, positions, weights=None):
     _weights(weights, tokens, k)
     dtype = T.float_type(grad, rows)
     dev = T.device()
-    gt, rt, pt = T.on(dev, grad, dtype), T.on(dev, rows, dtype), T.on(dev, positions, torch.int32)
+    gt, rt, pt = T.on(dev, grad, dtype), T.on(dev, rows, dtype), _places(dev, positions)
     wt = T.on(dev, weights, _weight_type(dtype))
     drows = torch.empty_like(rt)
     dweights = None
