@@ -364,8 +364,9 @@ GradLayout grad_layout(void *ws, int64_t n, int64_t d1, int64_t r, int64_t d2, i
     l.slot_off = c.take<int64_t>((size_t)r + 1);
     l.head = c.take<int64_t>(kHead);
     l.partial = nullptr;
-    if (dtype == BGL_BF16) {
-        // no tile is cut below kGradShortest slices
+    if (dtype == BGL_BF16 && n > kGradShortest * kGradSlice) {
+        // no sum of kGradShortest slices is cut; a longer one of L has at most
+        // ceil(L / kGradShortest) <= 2 (L - 1) / kGradShortest pieces
         int64_t slots = (int64_t)t.pairs * kGradSlots;
         const int64_t most = t.tiles1 * t.tiles2 * 2 * (n / kGradSlice) / kGradShortest;
         l.partial = c.take<float>((size_t)(slots < most ? slots : most) * kGradRows * kGradCols);
