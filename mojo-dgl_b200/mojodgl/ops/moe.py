@@ -106,7 +106,7 @@ def route_topk_backward(grad, logits, indices, *, score="softmax", renormalize=T
     itself, and so the bias, has no gradient.  Places with index -1 (any index
     that is not an expert's) have none either, nor have masked experts (logits of
     -inf) that a choice made elsewhere holds.  Returns (tokens, experts) in the
-    logits' type.
+    logits' type, float32 for float16 logits.
     """
     kind, (grad, logits, indices) = T.operands(grad, logits, indices)
     dtype = _logits(logits)

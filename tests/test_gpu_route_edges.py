@@ -1,5 +1,5 @@
 """Routing at its numeric ends: chosen experts that are masked, sigmoids that
-underflow.
+underflow; half-precision logits.
 
 u = 2^-24.  A weight loses |l| u of a logit l on its way into the exponential and
 a few u in sums and quotients of at most n terms: (n + 2 |l| + 16) u of its value;
@@ -100,3 +100,16 @@ def test_sigmoid_gradients_where_every_sigmoid_underflows():
     err = np.abs(got - want)
     tol = 2 * (12 + 2 * big + 16) * U * size
     assert (err <= tol + 2.0 ** -126).all(), (err - tol).max()
+
+
+@pytest.mark.parametrize("as_numpy", [False, True])
+def test_float16_logits_run_in_float32(as_numpy):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    logits, grad = torch.randn(30, 48, device="cuda", generator=g).half(), torch.randn(30, 5, device="cuda", generator=g)
+    give = (lambda t: t.cpu().numpy()) if as_numpy else (lambda t: t)
+    w, i = ops.route_topk(give(logits), 5)
+    want_w, want_i = ops.route_topk(logits.float(), 5)
+    back = ops.route_topk_backward(give(grad), give(logits), give(want_i))
+    want = ops.route_topk_backward(grad, logits.float(), want_i)
+    for got, ref in ((w, want_w), (i, want_i), (back, want)):
+        assert torch.equal(torch.as_tensor(got).cuda(), ref)
