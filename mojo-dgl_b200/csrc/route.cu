@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kMaxExperts = 1024, kMaxChoices = 32, kMaxGroups = 32;
 constexpr int kLanes = 8;            // lanes of a token
-constexpr int kSelect = 64;          // threads of a selecting block: one warp, so that SMs even out
+constexpr int kSelect = 64;          // threads of a selecting block: two warps, so that SMs even out
 constexpr int kSlots = kSelect / kLanes;  // its tokens
 constexpr int kWarps = 4;            // warps of a block of the backward pass
 
@@ -597,10 +597,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_route_topk_backward(const Route
 
 template <typename T, int SUBS, bool VEC>
 int launch_topk(const RouteArgs &a, cudaStream_t s) {
-    constexpr int most = kSlots * (select_row(SUBS) + kMaxChoices + kMaxGroups) * (int)sizeof(float);
-    if (most > 48 * 1024)
-        BGL_CUDA(cudaFuncSetAttribute(k_route_topk<T, SUBS, VEC>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    static_assert(kSlots * (select_row(SUBS) + kMaxChoices + kMaxGroups) * sizeof(float) <= 48 * 1024,
+                  "shared memory that every launch may have");
     const int64_t want = (a.tokens + kSlots - 1) / kSlots;
     k_route_topk<T, SUBS, VEC><<<(unsigned)(want < (1 << 20) ? want : 1 << 20), kSelect,
                                  kSlots * (select_row(SUBS) + a.k + a.groups) * sizeof(float), s>>>(a);
@@ -612,7 +610,7 @@ int launch_topk(const RouteArgs &a, cudaStream_t s) {
     const bool vec = a.experts % 4 == 0 && aligned(a.logits, 4 * sizeof(T));
     return vec ? launch_topk<T, SUBS, true>(a, s) : launch_topk<T, SUBS, false>(a, s);
 }
-// The fewest 32s (doubled) of experts that hold the row (a lane's registers grow with them).
+// The fewest sets of 64 experts, doubled, that hold the row (a lane's registers grow with them).
 template <typename T>
 int launch_topk(const RouteArgs &a, cudaStream_t s) {
     if (a.experts <= 8 * kLanes * 1) return launch_topk<T, 1>(a, s);
