@@ -253,9 +253,9 @@ int bgl_segment_mm_backward(const void *grad, const void *a, const void *b, cons
                             int64_t n, int64_t d1, int64_t r, int64_t d2, void *da, void *db,
                             int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Device-side status of the tensor-core grouped GEMM: 0, or the code of the
- * first bounded wait that expired (1-4) since the last call; synchronises
- * the device and clears the word. */
+/* Device-side status of the tensor-core grouped GEMMs: 0, or the code of the
+ * first bounded wait that expired since the last call (1-9; those of the
+ * gradient's kernel too); synchronises the device and clears the word. */
 int bgl_tc_error(void);
 
 /* ----------------------------------------- mixture-of-experts layer */
@@ -265,10 +265,11 @@ int bgl_tc_error(void);
  * Layer norm over the last axis of x (rows, d):
  *   y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias
  * weight and bias (d values) may be NULL, as may the outputs mean and rstd
- * (rows values each); y must not be x.  wdtype is dtype, or BGL_F32 for bf16 rows; mean and rstd
- * are float32, float64 for BGL_F64.  The backward call takes the mean and rstd
- * of the forward one; dx, dweight, dbias may be NULL (not computed), dweight and
- * dbias have wdtype.  The sums over rows have a fixed order. */
+ * (rows values each); y must not be x.  wdtype is dtype, or BGL_F32 for bf16
+ * rows; mean and rstd are float32, float64 for BGL_F64.  The backward call
+ * takes the mean and rstd of the forward one; dx, dweight, dbias may be NULL
+ * (not computed), dweight and dbias have wdtype.  The sums over rows have a
+ * fixed order. */
 int bgl_layer_norm(const void *x, const void *weight, const void *bias, int64_t rows, int64_t d,
                    double eps, void *y, void *mean, void *rstd, int dtype, int wdtype,
                    void *stream);

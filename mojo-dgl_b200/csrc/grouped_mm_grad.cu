@@ -164,7 +164,11 @@ __global__ void __launch_bounds__(1024)
 // thread (float64: 4 x 4), over strips of kDepth terms in two shared buffers: the
 // next strip is under way to registers while this one is multiplied.  32768 x 2048
 // x 1024 float32 over 16 segments: 7.3 ms for both gradients, of 3.8 ms that the
-// FMA pipes need (12.6 ms with 4 x 4 a thread and one buffer).
+// FMA pipes need (12.6 ms with 4 x 4 a thread and one buffer).  A sum over a segment's
+// rows is not cut here: where few segments of narrow blocks leave few tiles, db takes as
+// long as a block walks its rows (1000000 rows, float32, one segment of 64 x 64: 113 ms on
+// one block, five segments: 23 ms; bf16 of 60 x 60: 312 ms; bf16 of 64 x 64, on the tensor
+// cores, 0.19 ms).
 template <typename T>
 struct Simt {
     using A = Acc<T>;

@@ -411,9 +411,10 @@ __global__ void __launch_bounds__(threads_of(GROUP), forward_resident(GROUP, N, 
     if (far) recentre<GROUP>(x, w, b, first + threadIdx.x / GROUP, rows, stride, d, eps, y, mean, rstd, smem, turn);
 }
 
-// Blocks an SM that the backward pass is compiled for: what its registers allow
-// without spills (16384 x 4096 bf16: 89 us with two, 100 us with three; 131072 x
-// 256: 54 us with two, 49 us with three).
+// Blocks an SM that the backward pass is compiled for (16384 x 4096 bf16: 89 us with two,
+// 100 us with three; 131072 x 256: 54 us with two, 49 us with three).  Rows in aligned
+// pieces do so without spills; bf16 ones of 8 values a thread spill 20 to 32 bytes at
+// their 80 registers in the other modes, those of 16 values 48 to 72 by single values.
 __host__ __device__ constexpr int backward_resident(int group, int values, int size) {
     return group > kThreads || size == 8 ? 1 : values == 8 && size == 2 ? 3 : 2;
 }
@@ -800,7 +801,7 @@ int check_norm(const char *who, int64_t rows, int64_t d, int dtype, int wdtype) 
     return BGL_OK;
 }
 
-// Calls f with the group size, the values of a thread and VEC as constants.
+// Calls f with the group size and the values of a thread as constants.
 template <int GROUP, int N>
 struct Constant {
     static constexpr int group = GROUP, values = N;

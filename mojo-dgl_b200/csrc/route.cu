@@ -12,7 +12,7 @@
 // 172 us with a warp a token and scores rescanned every round, 92 us with 8 lanes
 // and every score in unrolled registers (code beyond the instruction cache), 62 us
 // with 4 lanes as below (fewest instructions, but 24 warps an SM and the last ones
-// run long), 51 us so.
+// run long), 51 us so (52.4 with the question whether every sigmoid underflows).
 //
 // A sigmoid of float32 accuracy costs 20 instructions, an approximate one 5.
 // Scores with a bias are therefore first taken from approximate sigmoids: where

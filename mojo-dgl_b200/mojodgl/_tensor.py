@@ -11,7 +11,8 @@ stay float32 (the B200 path); float64 stays float64 (the reference's own
 precision, ``python/mojodgl/_lib.py:127-163``); every other input goes through
 the reference's ``f64()`` rules -- complex is rejected, integers that float64
 cannot hold exactly are rejected, the rest widen to float64.  Half and bf16
-tensors compute in float32, except in segment_mm/gather_mm, which take bf16.
+tensors compute in float32, except where an operator takes bf16 as it is
+(segment_mm, gather_mm and the operators of a mixture-of-experts layer).
 """
 
 from __future__ import annotations

@@ -11,7 +11,8 @@ A mixture-of-experts layer on this package's grouped products::
 ``segment_mm_backward``, ``combine_backward`` and ``route_topk_backward`` lead
 back; the gradient of ``dispatch`` is ``combine`` without weights.  None of the
 functions here waits for the device (indices given as floats excepted, which are
-checked to be whole numbers).
+checked to be whole numbers), nor does ``segment_mm_backward``; ``segment_mm`` reads
+``counts`` back to check them.
 """
 
 from __future__ import annotations
