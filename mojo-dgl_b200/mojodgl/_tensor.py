@@ -167,6 +167,12 @@ def operands(*xs):
     return kind, xs
 
 
+# what ``feature`` makes of arrays of these types, whatever their values
+_FEATURE_TYPES = {torch.float32: torch.float32, torch.float64: torch.float64, torch.float16: torch.float32,
+                  torch.bfloat16: torch.float32, np.dtype(np.float32): torch.float32,
+                  np.dtype(np.float64): torch.float64}
+
+
 def is_bf16(a) -> bool:
     return isinstance(a, torch.Tensor) and a.dtype == torch.bfloat16
 
@@ -185,7 +191,8 @@ def float_type(*xs):
                 break
         else:
             return first
-    return common_float(*(feature(x) for x in xs))
+    types = [_FEATURE_TYPES.get(x.dtype) or feature(x).dtype for x in xs]  # (feature checks the others' values)
+    return torch.float32 if all(t in (torch.float32, np.float32) for t in types) else torch.float64
 
 
 def on(dev: torch.device, a, dtype: torch.dtype):
